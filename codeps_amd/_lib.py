@@ -7,7 +7,7 @@ library is missing `lib()` raises, and every op in codeps_amd goes through `lib(
 import ctypes
 import os
 import subprocess
-from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 
 import torch  # noqa: F401  (must precede loading the .so, see module docstring)
 
@@ -43,6 +43,17 @@ class ConvEpilogue(Structure):
 class ConvDesc(Structure):
     _fields_ = [(n, c_int32) for n in ("batch", "in_h", "in_w", "c0", "c1", "up0", "out_c", "out_h", "out_w", "kh", "kw",
                                        "stride", "pad", "pad_mode", "act", "stride_w", "pad_w", "pix_pitch", "row_pitch")]
+
+
+class ChannelNormDesc(Structure):
+    _fields_ = ([(n, c_int64) for n in ("rows", "x_pitch", "res_pitch", "gate_pitch", "dy_pitch", "dh_pitch")] +
+                [(n, c_int32) for n in ("channels", "rows_per_item", "full", "kind", "next_kind", "gate_mode", "gate_act", "x_type", "res_type",
+                                        "weight_type", "gate_type", "next_weight_type")] +
+                [(n, c_float) for n in ("scale", "eps", "next_eps")])
+
+
+class AdamWGroup(Structure):
+    _fields_ = [(n, c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_device", c_void_p)]
 
 
 def build(jobs=8, verbose=False):
@@ -183,6 +194,17 @@ SIGNATURES = {
     "codeps_panoptic_stats_workspace_bytes": (c_size_t, [I]),
     "codeps_panoptic_stats": (c_int, [P, P, I, I, I, I, I, I, P, P, P, P, c_size_t, P]),
     "codeps_adam_ema_step": (c_int, [P, P, P, P, P, LL, I, c_float, c_float, c_float, c_float, c_float, c_float, P]),
+    "codeps_channel_norm_fwd": (c_int, [POINTER(ChannelNormDesc), P, P, P, P, P, P, P, P, P, P, P]),
+    "codeps_channel_norm_bwd_workspace_bytes": (c_size_t, [POINTER(ChannelNormDesc)]),
+    "codeps_channel_norm_bwd": (c_int, [POINTER(ChannelNormDesc), P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, I, P, c_size_t, P]),
+    "codeps_adamw_item_bytes": (c_size_t, []),
+    "codeps_adamw_item_fill": (LL, [P, P, P, P, I, LL, I, LL, LL, I, LL]),
+    "codeps_adamw_workspace_bytes": (c_size_t, [I]),
+    "codeps_adamw_step": (c_int, [P, I, P, P, P, P, P, P, I, P, P, P, P, P, P, P, c_double, c_double, I, P, ctypes.c_ulonglong, c_double, P,
+                                  c_size_t, P]),
+    "codeps_adamw_moments_8bit": (c_int, [P, I, P, LL, P, P, P, P, P, P, P]),
+    "codeps_grad_norm_workspace_bytes": (c_size_t, [I]),
+    "codeps_grad_norm": (c_int, [P, P, P, I, c_double, P, P, c_size_t, P]),
     "codeps_ssim_fwd": (c_int, [P, P, I, I, I, c_float, c_float, P, P]),
     "codeps_ssim_bwd_workspace_bytes": (c_size_t, [I, I, I]),
     "codeps_ssim_bwd": (c_int, [P, P, P, I, I, I, c_float, c_float, P, P, P, c_size_t, P]),

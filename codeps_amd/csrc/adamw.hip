@@ -1,0 +1,543 @@
+// AdamW over many tensors at once and the global norm of their gradients.
+//   g' = g s c,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,  p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+// A step is two launches (four with clipping): a small one that advances every tensor's count t and turns it into the tensor's factors (64 bits: 1 - b2^t
+// of a young tensor loses its digits in 32), and the update itself.  Nothing of a step depends on host values but its scalars, so a captured step
+// replays as the next one.  The update reads and writes every byte once: 28 bytes per element with 32-bit states, 16 with 8-bit ones (fp32 gradients);
+// it is bound by bandwidth.
+//
+// Tensors are cut into chunks of 2048 elements, one block each; a table gives the tensor of a chunk.  The static part of a tensor (addresses, state
+// offsets) lies in a device table, gradient addresses travel in the launch's arguments: they change from step to step.
+//
+// 8-bit states: a wave owns a block of 256 elements (4 per lane), finds its largest magnitude (integer maximum of the bit patterns: NaN and infinity
+// win), takes the smallest power of two under which it fits, and rounds stochastically:
+//   q = floor(t / quantum + rho / 65536),  rho = 16 random bits
+// in integers: t 2^16 / quantum is below 2^21, its whole part plus rho is shifted by 16.  The fp32 value behind it is off by a unit at most, so the
+// result can differ from the exact one only where the sum lies within two units of a multiple of 65536: there (about 8 elements in 100 000) the
+// moments are formed again in 64 bits.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int CHUNK = 2048, QB = 256, THREADS = 256, PER_LAUNCH = 320;
+constexpr int MANT_M = 3, MANT_R = 4;
+constexpr int MAX_GROUPS = 16, PER_NORM = 160, NCHUNK = 4096, NORM_BLOCKS = 1024;
+
+struct Item {                                   // one tensor, in device memory
+    float* p;
+    float* ema;
+    void* copy;
+    long long n, off, packed;                   // elements; offset into the flat states (bits = 8: multiple of 256); offset among the 8-bit tensors, packed
+    long long chunk0;
+    int bits, copy_type, group, pad;
+};
+struct Factors {                                // of one tensor and step, in the workspace
+    double b1, ob1, b2, ob2, gs;                // 64 bits for the borders of the 8-bit codes
+    float fb1, fob1, fb2, fob2, fgs;
+    float keep, rate, root, eps;                // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), eps
+    unsigned k0, k1;                            // random keys
+    int live;                                   // 0: no gradient, or the step is skipped
+    int skipped;                                // the whole step is (nothing changes, EMA included)
+    int pad;
+};
+
+struct Grads {                                  // launch argument: the gradients of up to PER_LAUNCH tensors
+    const void* g[PER_LAUNCH];
+    unsigned char type[PER_LAUNCH];
+};
+struct NormTensors {                            // launch argument: the tensors one norm launch sums over
+    const void* g[PER_NORM];
+    long long n[PER_NORM];
+    unsigned chunk0[PER_NORM + 1];              // chunks of NCHUNK elements in front of a tensor
+    unsigned char type[PER_NORM];
+    int count;
+};
+struct Group { double lr, b1, b2, eps, wd; const float* lr_dev; };
+struct Groups { Group g[MAX_GROUPS]; unsigned live[(PER_LAUNCH + 31) / 32]; };
+
+__device__ __forceinline__ float grad_at(const void* g, int type, long long i) {
+    if (type == CODEPS_F32) return ((const float*)g)[i];
+    const unsigned short h = ((const unsigned short*)g)[i];
+    return type == CODEPS_BF16 ? __uint_as_float((unsigned)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+}
+// four gradients from i on; the ones from n on are zero
+__device__ __forceinline__ void grad4(const void* g, int type, long long i, long long n, float* o) {
+    if (i + 4 <= n) {
+        if (type == CODEPS_F32) {
+            const f32x4u q = *reinterpret_cast<const f32x4u*>((const float*)g + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = q[e];
+        } else {
+            const u16x4u q = *reinterpret_cast<const u16x4u*>((const unsigned short*)g + i);
+            if (type == CODEPS_BF16) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __uint_as_float((unsigned)q[e] << 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)q[e]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = i + e < n ? grad_at(g, type, i + e) : 0.f;
+    }
+}
+__device__ __forceinline__ void load4(const float* p, long long i, long long n, float* o) {
+    if (i + 4 <= n) {
+        const f32x4u q = *reinterpret_cast<const f32x4u*>(p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = q[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = i + e < n ? p[i + e] : 0.f;
+    }
+}
+__device__ __forceinline__ void store4(float* p, long long i, long long n, const float* v) {
+    if (i + 4 <= n) {
+        f32x4u q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = v[e];
+        *reinterpret_cast<f32x4u*>(p + i) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) p[i + e] = v[e];
+    }
+}
+__device__ __forceinline__ unsigned short narrow16(float v, int type) {
+    return type == CODEPS_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v) : __builtin_bit_cast(unsigned short, (_Float16)v);
+}
+__device__ __forceinline__ void store4_16(void* p, int type, long long i, long long n, const float* v) {
+    unsigned short* d = (unsigned short*)p + i;
+    if (i + 4 <= n) {
+        u16x4u q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = narrow16(v[e], type);
+        *reinterpret_cast<u16x4u*>(d) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) d[e] = narrow16(v[e], type);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ gradient norm
+// Sum of squares in 64 bits: an fp32 square overflows at 2e19, and sums over 10^8 elements lose digits.  A block walks a contiguous range of chunks, one
+// partial per block, added in a fixed order by the launch that needs the norm.
+__device__ __forceinline__ double block_sum64(double v, double* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+__global__ __launch_bounds__(THREADS) void grad_norm_kernel(NormTensors t, double* __restrict__ part) {
+    __shared__ double red[4];
+    const unsigned total = t.chunk0[t.count];
+    const unsigned c0 = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x), c1 = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
+    int lo = 0, hi = t.count - 1;                                  // the tensor of chunk c0: the last one that starts at or before it and is not empty
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.chunk0[mid] <= c0) lo = mid; else hi = mid - 1;
+    }
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (unsigned c = c0; c < c1; ++c) {
+        while (t.chunk0[lo + 1] <= c) ++lo;
+        const void* g = t.g[lo];
+        const long long n = t.n[lo], i0 = (long long)(c - t.chunk0[lo]) * NCHUNK + threadIdx.x * 4;
+        const int type = t.type[lo];
+        float v[NCHUNK / (THREADS * 4)][4];
+#pragma unroll
+        for (int k = 0; k < NCHUNK / (THREADS * 4); ++k) grad4(g, type, i0 + k * THREADS * 4, n, v[k]);
+#pragma unroll
+        for (int k = 0; k < NCHUNK / (THREADS * 4); ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += (double)v[k][e] * (double)v[k][e];
+    }
+    const double sum = block_sum64((s[0] + s[1]) + (s[2] + s[3]), red);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+
+__device__ __forceinline__ double norm_of(const double* part, int n_part, double scale, double* red) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n_part; i += THREADS) s += part[i];
+    return fabs(scale) * sqrt(block_sum64(s, red));
+}
+__global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(const double* __restrict__ part, int n_part, double scale, float* __restrict__ norm) {
+    __shared__ double red[4];
+    const double v = norm_of(part, n_part, scale, red);
+    if (threadIdx.x == 0) norm[0] = (float)v;
+}
+
+// ---------------------------------------------------------------------------------------------------------- a step's factors per tensor
+__global__ __launch_bounds__(THREADS) void adamw_factors_kernel(Groups groups, const Item* __restrict__ items, int base, int count, long long* __restrict__ steps,
+                                                                const double* __restrict__ part, int n_part, double grad_scale, double max_norm,
+                                                                int skip_nonfinite, float* __restrict__ norm_out, unsigned long long seed,
+                                                                Factors* __restrict__ out) {
+    __shared__ double red[4];
+    double gs = grad_scale;
+    bool skip = false;
+    if (n_part > 0) {
+        const double norm = norm_of(part, n_part, grad_scale, red);
+        if (max_norm > 0.0 && norm > max_norm) gs *= max_norm / norm;
+        skip = skip_nonfinite && !isfinite(norm);
+        if (norm_out && threadIdx.x == 0) norm_out[0] = (float)norm;
+    }
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+        const Group g = groups.g[items[base + i].group & (MAX_GROUPS - 1)];
+        const bool live = !skip && (groups.live[i >> 5] >> (i & 31) & 1);
+        long long t = steps[base + i];
+        if (live) steps[base + i] = ++t;
+        Factors f;
+        f.live = live; f.skipped = skip; f.pad = 0;
+        f.b1 = g.b1; f.ob1 = 1.0 - g.b1; f.b2 = g.b2; f.ob2 = 1.0 - g.b2; f.gs = gs;
+        f.fb1 = (float)f.b1; f.fob1 = (float)f.ob1; f.fb2 = (float)f.b2; f.fob2 = (float)f.ob2; f.fgs = (float)gs;
+        const double lr = g.lr_dev ? (double)*g.lr_dev : g.lr;
+        f.keep = (float)(1.0 - lr * g.wd);
+        f.rate = (float)(lr / (1.0 - pow(g.b1, (double)t)));
+        f.root = (float)(1.0 / sqrt(1.0 - pow(g.b2, (double)t)));
+        f.eps = (float)g.eps;
+        unsigned long long z = seed + (unsigned long long)t * 0x9E3779B97F4A7C15ull + (unsigned long long)(base + i) * 0xD1B54A32D192ED03ull;
+        z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+        z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+        z ^= z >> 31;
+        f.k0 = (unsigned)z; f.k1 = (unsigned)(z >> 32);
+        out[base + i] = f;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------------- 8-bit codes
+// Biased exponent of the block's unit for its largest magnitude (bit pattern): the next power of two when the mantissa would not fit below 2 - 2^-MANT.
+template <int MANT> __device__ __forceinline__ int unit_of(unsigned top) {
+    const unsigned e = (top + ((1u << (23 - MANT)) - 1)) >> 23;
+    return top < 0x00800000u ? 0 : (int)min(e, 255u);
+}
+// a code's bits, shifted to where fp32 has exponent and mantissa, are the value times 2^-112 -- field 0 included, as fp32's own subnormals
+template <int MANT> __device__ __forceinline__ float decode(unsigned code, int unit) {
+    return unit == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(__uint_as_float(code << (23 - MANT)), unit - 15);
+}
+template <int MANT, typename T> __device__ __forceinline__ int step_exponent(T a, int unit) {          // log2 of the quantum around a, in block units
+    const int e = a == (T)0 ? -14 : (sizeof(T) == 4 ? __builtin_amdgcn_frexp_expf((float)a) : __builtin_amdgcn_frexp_exp((double)a)) - 1 + 127 - unit;
+    return max(e, -14);
+}
+// |x| = a -> code.  slack: how far (in 2^-16 quanta) a may be from the exact value; unsure: whether that could change the code.
+template <int MANT> __device__ __forceinline__ unsigned encode(float a, int unit, unsigned rho, unsigned slack, bool& unsure) {
+    a = unit == 0 ? 0.f : a;
+    const int low = step_exponent<MANT, float>(a, unit);
+    const unsigned k = (unsigned)ldexpf(a, 127 - unit + MANT - low + 16) + rho;
+    unsure = ((k + slack) & 0xffffu) <= 2 * slack;
+    return ((unsigned)(low + 14) << MANT) + (k >> 16);
+}
+template <int MANT> __device__ __forceinline__ unsigned encode64(double a, int unit, unsigned rho) {
+    a = unit == 0 ? 0.0 : a;
+    const int low = step_exponent<MANT, double>(a, unit);
+    const unsigned k = (unsigned)ldexp(a, 127 - unit + MANT - low + 16) + rho;
+    return min(((unsigned)(low + 14) << MANT) + (k >> 16), (16u << MANT) - 1u);
+}
+__device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsigned k1) {
+    unsigned x = (unsigned)i + (unsigned)(i >> 32) * 0x9E3779B1u + k0;
+    x = (x ^ (x >> 16)) * 0x7FEB352Du;
+    x = x ^ (x >> 15) ^ k1;
+    x *= 0x846CA68Bu;
+    return x ^ (x >> 16);
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------ the update
+struct States { float *m, *v; unsigned char *mc, *me, *rc, *re; };
+
+__global__ __launch_bounds__(THREADS) void adamw_step_kernel(Grads grads, const Item* __restrict__ items, const int* __restrict__ chunk_items,
+                                                             const Factors* __restrict__ factors, int base, long long first_chunk, States st, float al, float oal) {
+    const long long chunk = first_chunk + blockIdx.x;
+    const int t = chunk_items[chunk];
+    const Item it = items[t];
+    const Factors& f = factors[t];
+    float* const ema = al >= 0.f ? it.ema : nullptr;
+    if (f.skipped || (!f.live && !ema)) return;
+    const long long n = it.n, start = (chunk - it.chunk0) * CHUNK;
+    constexpr int K = CHUNK / (THREADS * 4);
+    float p[K][4], g[K][4], a[K][4], b[K][4], em[K][4];
+    const void* gp = grads.g[t - base];
+    const int gt = grads.type[t - base];
+    const bool wide = it.bits == 32;
+    unsigned mc[K], rc[K];
+    int mu[K], ru[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = start + k * THREADS * 4 + threadIdx.x * 4;
+        load4(it.p, i, n, p[k]);
+        if (ema) load4(ema, i, n, em[k]);
+        if (!f.live) continue;
+        grad4(gp, gt, i, n, g[k]);
+        if (wide) {
+            load4(st.m + it.off, i, n, a[k]);
+            load4(st.v + it.off, i, n, b[k]);
+        } else if ((i & ~(long long)(QB - 1)) < n) {
+            const long long q = it.off + i;
+            mc[k] = *reinterpret_cast<const unsigned*>(st.mc + q);
+            rc[k] = *reinterpret_cast<const unsigned*>(st.rc + q);
+            mu[k] = st.me[q / QB];
+            ru[k] = st.re[q / QB];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = start + k * THREADS * 4 + threadIdx.x * 4;
+        if (f.live) {
+            if (wide) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float gg = g[k][e] * f.fgs;
+                    a[k][e] = f.fb1 * a[k][e] + f.fob1 * gg;
+                    b[k][e] = f.fb2 * b[k][e] + f.fob2 * gg * gg;
+                    p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(sqrtf(b[k][e]) * f.root + f.eps);
+                }
+                store4(st.m + it.off, i, n, a[k]);
+                store4(st.v + it.off, i, n, b[k]);
+            } else if ((i & ~(long long)(QB - 1)) < n) {                        // the same for a whole wave: it owns this block
+                float m0[4], r0[4];
+                unsigned mtop = 0, rtop = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned c = mc[k] >> (8 * e) & 255u;
+                    const float q = decode<MANT_M>(c & 127u, mu[k]);
+                    m0[e] = c & 128u ? -q : q;
+                    r0[e] = decode<MANT_R>(rc[k] >> (8 * e) & 255u, ru[k]);
+                    const float gg = g[k][e] * f.fgs;
+                    a[k][e] = f.fb1 * m0[e] + f.fob1 * gg;
+                    const float v = f.fb2 * (r0[e] * r0[e]) + f.fob2 * gg * gg;
+                    b[k][e] = sqrtf(v);
+                    p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(b[k][e] * f.root + f.eps);
+                    mtop = max(mtop, __float_as_uint(a[k][e]) & 0x7fffffffu);
+                    rtop = max(rtop, __float_as_uint(b[k][e]) & 0x7fffffffu);
+                }
+                mu[k] = unit_of<MANT_M>(wave_umax(mtop));
+                ru[k] = unit_of<MANT_R>(wave_umax(rtop));
+                unsigned ncm = 0, ncr = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned rnd = random_bits(i + e, f.k0, f.k1);
+                    bool um, ur;
+                    // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
+                    const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(f.fob1 * g[k][e] * f.fgs);
+                    const int low = step_exponent<MANT_M, float>(mu[k] == 0 ? 0.f : am, mu[k]);
+                    const unsigned slack = 2u + (unsigned)fminf(ldexpf(size, 127 - mu[k] + MANT_M - low + 16 - 22), 32000.f);
+                    unsigned cm = encode<MANT_M>(am, mu[k], rnd & 0xffffu, slack, um);
+                    unsigned cr = encode<MANT_R>(b[k][e], ru[k], rnd >> 16, 2u, ur);
+                    if (um || ur) {
+                        const double gg = (double)g[k][e] * f.gs;
+                        if (um) cm = encode64<MANT_M>(fabs(f.b1 * (double)m0[e] + f.ob1 * gg), mu[k], rnd & 0xffffu);
+                        if (ur) cr = encode64<MANT_R>(sqrt(f.b2 * ((double)r0[e] * (double)r0[e]) + f.ob2 * gg * gg), ru[k], rnd >> 16);
+                    }
+                    ncm |= ((mu[k] == 255 ? 0u : cm & 127u) | (a[k][e] < 0.f ? 128u : 0u)) << (8 * e);
+                    ncr |= (ru[k] == 255 ? 0u : cr & 255u) << (8 * e);
+                }
+                const long long q = it.off + i;
+                *reinterpret_cast<unsigned*>(st.mc + q) = ncm;
+                *reinterpret_cast<unsigned*>(st.rc + q) = ncr;
+                if ((threadIdx.x & 63) == 0) {
+                    st.me[q / QB] = (unsigned char)mu[k];
+                    st.re[q / QB] = (unsigned char)ru[k];
+                }
+            }
+            store4(it.p, i, n, p[k]);
+            if (it.copy) store4_16(it.copy, it.copy_type, i, n, p[k]);
+        }
+        if (ema) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) em[k][e] = al * em[k][e] + oal * p[k][e];
+            store4(ema, i, n, em[k]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void adamw_moments_kernel(const Item* __restrict__ items, const int* __restrict__ chunk_items, const unsigned char* __restrict__ mc,
+                                                                const unsigned char* __restrict__ me, const unsigned char* __restrict__ rc,
+                                                                const unsigned char* __restrict__ re, void* __restrict__ om, void* __restrict__ orr) {
+    const long long chunk = blockIdx.x;
+    const Item it = items[chunk_items[chunk]];
+    if (it.bits != 8) return;
+    const long long n = it.n, start = (chunk - it.chunk0) * CHUNK;
+#pragma unroll
+    for (int k = 0; k < CHUNK / (THREADS * 4); ++k) {
+        const long long i = start + k * THREADS * 4 + threadIdx.x * 4, q = it.off + i;
+        if (i >= n) continue;
+        const unsigned cm = *reinterpret_cast<const unsigned*>(mc + q), cr = *reinterpret_cast<const unsigned*>(rc + q);
+        const int mu = me[q / QB], ru = re[q / QB];
+        float m[4], r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned c = cm >> (8 * e) & 255u;
+            const float v = decode<MANT_M>(c & 127u, mu);
+            m[e] = c & 128u ? -v : v;
+            r[e] = decode<MANT_R>(cr >> (8 * e) & 255u, ru);
+        }
+        store4_16((unsigned short*)om + it.packed, CODEPS_BF16, i, n, m);
+        store4_16((unsigned short*)orr + it.packed, CODEPS_BF16, i, n, r);
+    }
+}
+
+bool grad_type_ok(int t) { return t == CODEPS_F32 || t == CODEPS_BF16 || t == CODEPS_F16; }
+
+// partial sums of squares of all tensors into `part`; the number of partials, or a negative code
+int norm_partials(const void* const* grads, const unsigned char* types, const long long* numels, int n, double* part, hipStream_t st) {
+    int parts = 0;
+    for (int base = 0; base < n;) {
+        NormTensors t;
+        t.count = 0;
+        long long chunks = 0;
+        while (base < n && t.count < PER_NORM) {
+            const long long c = grads[base] ? (numels[base] + NCHUNK - 1) / NCHUNK : 0;
+            if (chunks + c > 0xffffffffLL) break;
+            t.g[t.count] = grads[base]; t.n[t.count] = numels[base]; t.type[t.count] = types[base];
+            t.chunk0[t.count++] = (unsigned)chunks;
+            chunks += c;
+            ++base;
+        }
+        t.chunk0[t.count] = (unsigned)chunks;
+        if (chunks == 0) continue;
+        const int blocks = (int)std::min<long long>(chunks, NORM_BLOCKS);
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(THREADS), 0, st, t, part + parts);
+        CODEPS_CHECK_LAUNCH("grad_norm_kernel");
+        parts += blocks;
+    }
+    return parts;
+}
+size_t norm_bytes(int n) { return (size_t)cdiv(n, PER_NORM) * NORM_BLOCKS * sizeof(double); }
+
+int check_grads(const void* const* grads, const unsigned char* types, const long long* numels, int n, const char* who) {
+    CODEPS_REQUIRE(grads && types && numels && n >= 1 && n <= (1 << 24), CODEPS_ERR_ARG, "%s: null array, or not 1 .. 2^24 tensors", who);
+    for (int i = 0; i < n; ++i) {
+        CODEPS_REQUIRE(numels[i] >= 0 && numels[i] <= (1LL << 40), CODEPS_ERR_ARG, "%s: tensor %d has %lld elements", who, i, numels[i]);
+        CODEPS_REQUIRE(!grads[i] || grad_type_ok(types[i]), CODEPS_ERR_ARG, "%s: gradient %d has the unknown type %d", who, i, (int)types[i]);
+        CODEPS_REQUIRE(((uintptr_t)grads[i] & (types[i] == CODEPS_F32 ? 3 : 1)) == 0, CODEPS_ERR_ARG, "%s: gradient %d is not aligned to its elements", who, i);
+    }
+    return CODEPS_OK;
+}
+
+}  // namespace
+
+// =============================================================================================== C ABI
+extern "C" size_t codeps_adamw_item_bytes(void) { return sizeof(Item); }
+
+extern "C" long long codeps_adamw_item_fill(void* item, float* param, float* ema, void* copy, int copy_type, long long numel, int bits,
+                                            long long state_offset, long long packed_offset, int group, long long chunk0) {
+    CODEPS_REQUIRE(item && (param || numel == 0) && numel >= 0 && numel <= (1LL << 40), CODEPS_ERR_ARG, "adamw_item_fill: null pointer or bad element count");
+    CODEPS_REQUIRE(bits == 32 || bits == 8, CODEPS_ERR_ARG, "adamw_item_fill: states have 32 or 8 bits, not %d", bits);
+    CODEPS_REQUIRE(state_offset >= 0 && packed_offset >= 0 && chunk0 >= 0 && (bits == 32 || state_offset % QB == 0), CODEPS_ERR_ARG,
+                   "adamw_item_fill: state offset %lld (8-bit states start at multiples of %d)", state_offset, QB);
+    CODEPS_REQUIRE(group >= 0 && group < MAX_GROUPS, CODEPS_ERR_ARG, "adamw_item_fill: group %d of at most %d", group, MAX_GROUPS);
+    CODEPS_REQUIRE(!copy || copy_type == CODEPS_BF16 || copy_type == CODEPS_F16, CODEPS_ERR_ARG, "adamw_item_fill: a copy is bf16 or fp16");
+    CODEPS_REQUIRE((((uintptr_t)param | (uintptr_t)ema) & 3) == 0 && ((uintptr_t)copy & 1) == 0, CODEPS_ERR_ARG, "adamw_item_fill: unaligned pointer");
+    const Item it = {param, ema, copy, numel, state_offset, packed_offset, chunk0, bits, copy_type, group, 0};
+    memcpy(item, &it, sizeof(it));
+    return (numel + CHUNK - 1) / CHUNK;
+}
+
+extern "C" size_t codeps_adamw_workspace_bytes(int n_items) {
+    if (n_items < 1) { codeps_set_error("adamw_workspace_bytes: %d tensors", n_items); return 0; }
+    return align_up((size_t)n_items * sizeof(Factors), 256) + norm_bytes(n_items);
+}
+
+extern "C" int codeps_adamw_step(const void* items, int n_items, const int* chunk_items, const long long* chunk0, const void* const* grads,
+                                 const unsigned char* grad_types, const long long* numels, const codeps_adamw_group* groups, int n_groups,
+                                 long long* steps, float* exp_avg, float* exp_avg_sq, unsigned char* exp_avg_codes, unsigned char* exp_avg_exponents,
+                                 unsigned char* root_codes, unsigned char* root_exponents, double grad_scale, double max_norm, int skip_nonfinite,
+                                 float* norm, unsigned long long seed, double ema_alpha, void* workspace, size_t workspace_bytes,
+                                 codeps_stream_t stream) {
+    const int rc = check_grads(grads, grad_types, numels, n_items, "adamw_step");
+    if (rc != CODEPS_OK) return rc;
+    CODEPS_REQUIRE(items && chunk_items && chunk0 && steps && groups && workspace, CODEPS_ERR_ARG, "adamw_step: null pointer");
+    CODEPS_REQUIRE(n_groups >= 1 && n_groups <= MAX_GROUPS, CODEPS_ERR_ARG, "adamw_step: %d groups (1 .. %d)", n_groups, MAX_GROUPS);
+    CODEPS_REQUIRE(workspace_bytes >= codeps_adamw_workspace_bytes(n_items), CODEPS_ERR_WORKSPACE, "adamw_step: %zu bytes of workspace, %zu are needed",
+                   workspace_bytes, codeps_adamw_workspace_bytes(n_items));
+    CODEPS_REQUIRE((exp_avg == nullptr) == (exp_avg_sq == nullptr) && (exp_avg_codes == nullptr) == (root_codes == nullptr) &&
+                   (exp_avg_codes == nullptr) == (exp_avg_exponents == nullptr) && (exp_avg_codes == nullptr) == (root_exponents == nullptr) &&
+                   (exp_avg || exp_avg_codes), CODEPS_ERR_ARG, "adamw_step: incomplete states");
+    for (int i = 0; i < n_groups; ++i) {
+        const codeps_adamw_group& g = groups[i];
+        CODEPS_REQUIRE(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0, CODEPS_ERR_ARG,
+                       "adamw_step: group %d has betas (%g, %g), eps %g", i, g.beta1, g.beta2, g.eps);
+    }
+    for (int i = 0; i < n_items; ++i)
+        CODEPS_REQUIRE(chunk0[i + 1] - chunk0[i] == (numels[i] + CHUNK - 1) / CHUNK, CODEPS_ERR_ARG, "adamw_step: tensor %d: chunk table and element count differ", i);
+    hipStream_t st = (hipStream_t)stream;
+    Factors* factors = (Factors*)workspace;
+    double* part = (double*)((char*)workspace + align_up((size_t)n_items * sizeof(Factors), 256));
+    int parts = 0;
+    if (max_norm > 0.0 || skip_nonfinite || norm) {
+        parts = norm_partials(grads, grad_types, numels, n_items, part, st);
+        if (parts < 0) return parts;
+    }
+    Groups gs;
+    for (int i = 0; i < MAX_GROUPS; ++i) {
+        const codeps_adamw_group& g = groups[std::min(i, n_groups - 1)];
+        gs.g[i] = {g.lr, g.beta1, g.beta2, g.eps, g.weight_decay, g.lr_device};
+    }
+    const States states = {exp_avg, exp_avg_sq, exp_avg_codes, exp_avg_exponents, root_codes, root_exponents};
+    for (int base = 0; base < n_items; base += PER_LAUNCH) {
+        const int count = std::min(PER_LAUNCH, n_items - base);
+        memset(gs.live, 0, sizeof(gs.live));
+        Grads gr;
+        for (int i = 0; i < count; ++i) {
+            gr.g[i] = grads[base + i];
+            gr.type[i] = grad_types[base + i];
+            if (grads[base + i]) gs.live[i >> 5] |= 1u << (i & 31);
+        }
+        // (without gradients at all there are no partials: the norm is 0)
+        if (parts == 0 && norm && base == 0) {
+            hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, st, (const double*)part, 0, grad_scale, norm);
+            CODEPS_CHECK_LAUNCH("grad_norm_finish_kernel");
+        }
+        hipLaunchKernelGGL(adamw_factors_kernel, dim3(1), dim3(THREADS), 0, st, gs, (const Item*)items, base, count, steps, (const double*)part, parts,
+                           grad_scale, max_norm, skip_nonfinite, norm, seed, factors);
+        CODEPS_CHECK_LAUNCH("adamw_factors_kernel");
+        long long first = chunk0[base];
+        const long long end = chunk0[base + count];
+        for (; first < end; first += 1LL << 30) {
+            hipLaunchKernelGGL(adamw_step_kernel, dim3((unsigned)std::min<long long>(end - first, 1LL << 30)), dim3(THREADS), 0, st, gr, (const Item*)items,
+                               chunk_items, (const Factors*)factors, base, first, states, (float)ema_alpha, (float)(1.0 - ema_alpha));
+            CODEPS_CHECK_LAUNCH("adamw_step_kernel");
+        }
+    }
+    return CODEPS_OK;
+}
+
+extern "C" int codeps_adamw_moments_8bit(const void* items, int n_items, const int* chunk_items, long long n_chunks, const unsigned char* exp_avg_codes,
+                                         const unsigned char* exp_avg_exponents, const unsigned char* root_codes, const unsigned char* root_exponents,
+                                         void* exp_avg_bf16, void* root_bf16, codeps_stream_t stream) {
+    CODEPS_REQUIRE(items && n_items >= 1 && chunk_items && n_chunks >= 1 && n_chunks < (1LL << 31) && exp_avg_codes && exp_avg_exponents && root_codes &&
+                   root_exponents && exp_avg_bf16 && root_bf16, CODEPS_ERR_ARG, "adamw_moments_8bit: bad arguments");
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)n_chunks), dim3(THREADS), 0, (hipStream_t)stream, (const Item*)items, chunk_items, exp_avg_codes,
+                       exp_avg_exponents, root_codes, root_exponents, exp_avg_bf16, root_bf16);
+    CODEPS_CHECK_LAUNCH("adamw_moments_kernel");
+    return CODEPS_OK;
+}
+
+extern "C" size_t codeps_grad_norm_workspace_bytes(int n_tensors) {
+    if (n_tensors < 1) { codeps_set_error("grad_norm_workspace_bytes: %d tensors", n_tensors); return 0; }
+    return norm_bytes(n_tensors);
+}
+
+extern "C" int codeps_grad_norm(const void* const* grads, const unsigned char* grad_types, const long long* numels, int n_tensors, double scale,
+                                float* norm, void* workspace, size_t workspace_bytes, codeps_stream_t stream) {
+    const int rc = check_grads(grads, grad_types, numels, n_tensors, "grad_norm");
+    if (rc != CODEPS_OK) return rc;
+    CODEPS_REQUIRE(norm && workspace && workspace_bytes >= norm_bytes(n_tensors), CODEPS_ERR_WORKSPACE, "grad_norm: null pointer or workspace too small");
+    hipStream_t st = (hipStream_t)stream;
+    const int parts = norm_partials(grads, grad_types, numels, n_tensors, (double*)workspace, st);
+    if (parts < 0) return parts;
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, st, (const double*)workspace, parts, scale, norm);
+    CODEPS_CHECK_LAUNCH("grad_norm_finish_kernel");
+    return CODEPS_OK;
+}

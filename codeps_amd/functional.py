@@ -2342,6 +2342,212 @@ def weighted_sum(losses, weights, factors=None, denom=None):
     return _WeightedSum.apply(list(weights), None if factors is None else list(factors), denom, *losses)
 
 
+# ---------------------------------------------------------------------------------------- channel norms (C ABI: codeps_channel_norm_*)
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+_GATE_ACTS = {None: 0, "sigmoid": 1, "silu": 2}
+_MAX_NORM_CHANNELS = 8192
+
+
+class _OnDevice:
+    """Makes the tensors' device the current one for the launches inside (nothing to do when it is: torch.cuda.device costs microseconds)."""
+
+    def __init__(self, device):
+        self.scope = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.scope is not None:
+            self.scope.__enter__()
+
+    def __exit__(self, *exc):
+        if self.scope is not None:
+            self.scope.__exit__(*exc)
+
+
+def _pitched(t):
+    """(tensor, elements from row to row): t itself when its channels are dense and its rows lie at one distance, else a contiguous copy."""
+    c = t.shape[-1]
+    if t.is_contiguous():
+        return t, c
+    if t.stride(-1) == 1 or c == 1:
+        pitch, span = None, 1
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch is None:
+                pitch = stride
+            elif stride != pitch * span:
+                pitch = -1
+                break
+            span *= size
+        if pitch is None:
+            return t, c
+        if pitch >= c:
+            return t, pitch
+    return t.contiguous(), c
+
+
+def _vector(v, c, what, device):
+    if v is None:
+        return None
+    if v.dim() != 1 or v.shape[0] != c or v.dtype not in _TYPES or v.device != device:
+        raise CodepsHipError(f"{what}: one value per channel ({c}) in fp32, bf16 or fp16 on {device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
+    return v.contiguous()
+
+
+class _ChannelNorm(torch.autograd.Function):
+    """Both public forms.  cfg = (full, kind, eps, gate mode, gate activation, rows per item, scale, next kind, next eps)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, gate, weight, bias, next_weight, next_bias, cfg):
+        full, kind, eps, mode, act, per_item, scale, nkind, neps = cfg
+        c = x.shape[-1]
+        d = _lib.ChannelNormDesc()
+        d.rows, d.channels, d.rows_per_item, d.full = x.numel() // c, c, per_item, full
+        d.kind, d.next_kind, d.gate_mode, d.gate_act = kind, nkind, mode, act
+        d.x_type = _TYPES[x.dtype]
+        xr, d.x_pitch = _pitched(x)
+        d.res_type, d.res_pitch = d.x_type, c
+        rr = None
+        if residual is not None:
+            rr, d.res_pitch = _pitched(residual)
+            d.res_type = _TYPES[residual.dtype]
+        gr = None
+        if gate is not None:
+            gr, d.gate_pitch = _pitched(gate)
+            d.gate_type = _TYPES[gate.dtype]
+        vec = weight if weight is not None else bias
+        d.weight_type = 0 if vec is None else _TYPES[vec.dtype]
+        vec = next_weight if next_weight is not None else next_bias
+        d.next_weight_type = 0 if vec is None else _TYPES[vec.dtype]
+        d.scale, d.eps, d.next_eps = scale, eps, neps
+        y = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device) if full else None
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if (nkind or not full) else None
+        stats = torch.empty(d.rows, 4 if full else 2, dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
+        with _OnDevice(x.device):
+            check(lib().codeps_channel_norm_fwd(ctypes.byref(d), ptr(xr), ptr(rr), ptr(gr), ptr(weight), ptr(bias), ptr(next_weight), ptr(next_bias),
+                                                ptr(y), ptr(h), ptr(stats), stream_ptr()), "codeps_channel_norm_fwd")
+        if stats is not None:
+            ctx.save_for_backward(xr, rr if nkind else None, gr, weight, bias, next_weight, stats)
+            ctx.d, ctx.gate_shape, ctx.res_dtype = d, None if gate is None else gate.shape, None if residual is None else residual.dtype
+            vectors = (weight, bias, next_weight, next_bias)
+            ctx.vec_dtypes = [None if v is None else v.dtype for v in vectors]
+            ctx.sinks = [grad_sink(v) if v is not None and v.requires_grad else None for v in vectors]     # (flat-gradient views: fp32, contiguous)
+        ctx.set_materialize_grads(False)
+        if full:
+            return (y, h) if nkind else y
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *douts):
+        x, residual, gate, weight, bias, next_weight, stats = ctx.saved_tensors
+        d0 = ctx.d
+        d = type(d0).from_buffer_copy(d0)             # (two backward passes of one forward may run at once)
+        c, dev, need = d.channels, x.device, ctx.needs_input_grad
+        dy, dh = (douts[0], douts[1] if d.next_kind else None) if d.full else (None, douts[0])
+        if dy is None and dh is None:
+            return (None,) * 8
+        if dy is not None:
+            dy, d.dy_pitch = _pitched(dy)
+        if dh is not None:
+            dh, d.dh_pitch = _pitched(dh)
+        elif d.next_kind:                             # h is not part of the loss: the block's end alone
+            d.next_kind = 0
+            residual = None
+        empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)                     # noqa: E731
+        dx = empty(x.shape, x.dtype) if need[0] else None
+        dres = empty(x.shape, ctx.res_dtype) if need[1] else None
+        dgate = (empty if d.rows else lambda s, t: torch.zeros(s, dtype=t, device=dev))(ctx.gate_shape, gate.dtype) if need[2] else None
+        outs, acc = [], 0
+        for i in range(4):
+            out = None
+            if need[3 + i] and (i < 2 or d.next_kind):
+                out = ctx.sinks[i]
+                if out is not None:
+                    acc |= 1 << i
+                else:
+                    out = empty((c,), ctx.vec_dtypes[i])
+            outs.append(out)
+        with _OnDevice(dev):
+            nbytes = lib().codeps_channel_norm_bwd_workspace_bytes(ctypes.byref(d))
+            if nbytes == 0:
+                check(-1, "codeps_channel_norm_bwd_workspace_bytes")
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)      # not a cached one: captured graphs must not share it
+            check(lib().codeps_channel_norm_bwd(ctypes.byref(d), ptr(x), ptr(residual), ptr(gate), ptr(weight), ptr(bias), ptr(next_weight), ptr(stats),
+                                                ptr(dy), ptr(dh), ptr(dx), ptr(dres), ptr(dgate), ptr(outs[0]), ptr(outs[1]), ptr(outs[2]), ptr(outs[3]),
+                                                acc, ptr(ws), nbytes, stream_ptr()), "codeps_channel_norm_bwd")
+        return (dx, dres, dgate) + tuple(None if ctx.sinks[i] is not None else outs[i] for i in range(4)) + (None,)
+
+
+def _check_rows(x, what):
+    require_cuda(x)
+    if x.dtype not in _TYPES:
+        raise CodepsHipError(f"{what}: fp32, bf16 or fp16, got {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_NORM_CHANNELS:
+        raise CodepsHipError(f"{what}: [..., channels] with 1 .. {_MAX_NORM_CHANNELS} channels, got {tuple(x.shape)}")
+    return x.shape[-1]
+
+
+def _check_norm(kind, weight, bias, eps, c, what, device):
+    if kind not in _NORM_KINDS:
+        raise CodepsHipError(f"{what}: kind is \"layer\", \"rms\" or None, got {kind!r}")
+    if not eps >= 0.0:
+        raise CodepsHipError(f"{what}: eps = {eps}")
+    weight, bias = _vector(weight, c, what + ": weight", device), _vector(bias, c, what + ": bias", device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise CodepsHipError(f"{what}: weight ({weight.dtype}) and bias ({bias.dtype}) have one type")
+    return weight, bias
+
+
+def channel_norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
+    """Norm over the last dimension of x [..., C], the channels of a pixel (NHWC) or token:  n(x) weight + bias  with
+    n(x) = (x - mean) / sqrt(var + eps)  ("layer")  or  x / sqrt(mean x^2 + eps)  ("rms").  fp32, bf16 or fp16; the statistics are fp32.  weight, bias
+    [C]: one type of the three, their gradients are summed in fp32 in a fixed order.  x may be a channel slice of a wider (padded) map: rows are read
+    where they lie.  Unlike F.batch_norm_train it does not depend on the other items of the batch."""
+    c = _check_rows(x, "channel_norm")
+    if kind is None:
+        raise CodepsHipError("channel_norm: kind is \"layer\" or \"rms\"")
+    weight, bias = _check_norm(kind, weight, bias, eps, c, "channel_norm", x.device)
+    return _ChannelNorm.apply(x, None, None, weight, bias, None, None, (0, _NORM_KINDS[kind], eps, 0, 0, 1, 1.0, 0, 0.0))
+
+
+def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=None, gate_act=None, scale=1.0, next_kind=None,
+                          next_weight=None, next_bias=None, next_eps=1e-5):
+    """The end of a residual block and the norm in front of the next one, in one pass over the rows:
+        y = residual + scale act(gate) (n(x) weight + bias),   h = n'(y) next_weight + next_bias
+    Returns y, or (y, h) with next_kind.  x [..., C] is the block's output; kind None leaves it as it is (times weight, plus bias, if given).
+    residual: x's shape, x's type or fp32 (a residual stream in 32 bits around 16-bit blocks); y has its type, h has x's.  None: zeros.
+    gate: [C] (layer scale), one row per item of the first dimension ([B, C], or x's number of dimensions with ones in between), or x's shape;
+    gate_act: None, "sigmoid" or "silu".  scale: a float.  h is the norm of y before y is rounded to its type."""
+    what = "channel_norm_residual"
+    c = _check_rows(x, what)
+    weight, bias = _check_norm(kind, weight, bias, eps, c, what, x.device)
+    next_weight, next_bias = _check_norm(next_kind, next_weight, next_bias, next_eps, c, what + " (next)", x.device)
+    if next_kind is None and (next_weight is not None or next_bias is not None):
+        raise CodepsHipError(f"{what}: next_weight / next_bias without next_kind")
+    if residual is not None:
+        if residual.shape != x.shape or residual.device != x.device or residual.dtype not in (x.dtype, torch.float32):
+            raise CodepsHipError(f"{what}: residual has x's shape and device, and x's type or fp32: got {tuple(residual.shape)} {residual.dtype} on "
+                                 f"{residual.device} for {tuple(x.shape)} {x.dtype} on {x.device}")
+    if gate_act not in _GATE_ACTS or (gate is None and gate_act is not None):
+        raise CodepsHipError(f"{what}: gate_act is None, \"sigmoid\" or \"silu\", and goes with a gate: got {gate_act!r}")
+    mode, per_item = 0, 1
+    if gate is not None:
+        if gate.dtype not in _TYPES or gate.device != x.device or gate.dim() < 1 or gate.shape[-1] != c:
+            raise CodepsHipError(f"{what}: gate [..., {c}] in fp32, bf16 or fp16 on {x.device}, got {tuple(gate.shape)} {gate.dtype} on {gate.device}")
+        if gate.dim() == 1:
+            mode = 1
+        elif gate.shape == x.shape:
+            mode = 3
+        elif (gate.dim() == 2 or gate.dim() == x.dim()) and gate.shape[0] == x.shape[0] and gate.numel() == gate.shape[0] * c and x.dim() > 2:
+            mode, per_item = 2, max(1, x.numel() // c // max(1, x.shape[0]))
+        else:
+            raise CodepsHipError(f"{what}: gate is [{c}], one row per item of x's first dimension, or x's shape: got {tuple(gate.shape)} for {tuple(x.shape)}")
+    return _ChannelNorm.apply(x, residual, gate, weight, bias, next_weight, next_bias,
+                              (1, _NORM_KINDS[kind], eps, mode, _GATE_ACTS[gate_act], per_item, float(scale), _NORM_KINDS[next_kind], next_eps))
+
+
 # ---------------------------------------------------------------------------------------- optimiser
 def adam_ema_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, grad_scale=1.0,
                   ema_params=None, ema_alpha=0.99):
@@ -2351,6 +2557,42 @@ def adam_ema_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-4, betas=(0.9,
                                      int(step), lr, betas[0], betas[1], eps, grad_scale, ema_alpha, stream_ptr()),
           "codeps_adam_ema_step")
     invalidate_weight_cache()
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, in any order of its dimensions (contiguous, channels-last, ...)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def grad_norm(grads, scale=1.0):
+    """|scale g|_2 over a list of gradients (None entries are skipped), fp32 on the device: what AdamW clips by (C ABI: codeps_grad_norm).  fp32, bf16 and
+    fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise CodepsHipError("grad_norm: no gradients")
+    dev = grads[0].device
+    require_cuda(grads[0])
+    for i, g in enumerate(grads):
+        if g.dtype not in _TYPES or g.device != dev:
+            raise CodepsHipError(f"grad_norm: fp32, bf16 or fp16 tensors on one device, got {g.dtype} on {g.device}")
+        if not g.is_contiguous() and not _dense(g):
+            grads[i] = g.contiguous()
+    n = len(grads)
+    out = torch.empty((), dtype=torch.float32, device=dev)
+    with _OnDevice(dev):
+        nbytes = lib().codeps_grad_norm_workspace_bytes(n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        check(lib().codeps_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_ubyte * n)(*[_TYPES[g.dtype] for g in grads]),
+                                     (ctypes.c_longlong * n)(*[g.numel() for g in grads]), n, float(scale), ptr(out), ptr(ws), nbytes, stream_ptr()),
+              "codeps_grad_norm")
+    return out
 
 
 # ---------------------------------------------------------------------------------------- panoptic fusion

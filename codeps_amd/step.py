@@ -2,7 +2,8 @@
 one pre-training step (scripts/train_codeps.py:97-108).
 
     zero flat grads -> CodepsNet forward (adapt / train) -> sum_k w_k loss_k -> backward
-    -> ONE all-reduce of the flat gradient buffer (world > 1) -> fused Adam (+ EMA teacher) on flat buffers
+    -> ONE all-reduce of the flat gradient buffer (world > 1) -> fused Adam (+ EMA teacher) on flat buffers, or AdamW over all
+       parameters (cfg.train.optimizer.type "AdamW": decoupled decay, clipping, 8-bit states; codeps_amd.optim)
 
 All trainable parameters live in ONE flat fp32 buffer (views handed back to the nn.Parameters), likewise
 their gradients, Adam moments and the EMA copy; conv weight / bias gradients are accumulated straight into
@@ -55,17 +56,17 @@ def ema_module_lists(cfg, frozen):
 class FlatState:
     """Flat parameter / gradient / Adam / EMA buffers over a list of parameters."""
 
-    def __init__(self, params, with_ema, grad=None):
+    def __init__(self, params, with_ema, grad=None, moments=True):
         """grad: this group's slice of the step's ONE flat gradient buffer (StepRunner.grad_all), so that the whole step has a
-        single all-reduce; None allocates a private buffer."""
+        single all-reduce; None allocates a private buffer.  moments False: no Adam moments (another optimizer keeps its own)."""
         self.params = params
         n = sum(p.numel() for p in params)
         dev = params[0].device
         self.flat = torch.empty(n, dtype=torch.float32, device=dev)
         self.grad = torch.zeros(n, dtype=torch.float32, device=dev) if grad is None else grad
         assert self.grad.numel() == n and self.grad.is_contiguous()
-        self.m = torch.zeros(n, dtype=torch.float32, device=dev)
-        self.v = torch.zeros(n, dtype=torch.float32, device=dev)
+        self.m = torch.zeros(n, dtype=torch.float32, device=dev) if moments else None
+        self.v = torch.zeros(n, dtype=torch.float32, device=dev) if moments else None
         off = 0
         for p in params:
             k = p.numel()
@@ -169,10 +170,12 @@ class StepRunner:
         total = sum(p.numel() for ps, _ in sets for p in ps)
         self.grad_all = torch.zeros(total, dtype=torch.float32, device=sets[0][0][0].device)
         self.groups, off = [], 0
+        adamw = cfg.train.optimizer.get("type", "Adam") == "AdamW"
         for ps, with_ema in sets:
             n = sum(p.numel() for p in ps)
-            self.groups.append(FlatState(ps, with_ema, self.grad_all[off:off + n]))
+            self.groups.append(FlatState(ps, with_ema, self.grad_all[off:off + n], moments=not adamw))
             off += n
+        self.adamw = self._make_adamw(cfg.train.optimizer) if adamw else None
         self.step_count = 0
         # ---- world > 1: the gradient all-reduce in two segments.  Segment A = the EMA'd modules + the other heads (the flat buffer's
         # front), launched on its own stream from inside the backward pass as soon as the last kernel that writes it has been issued
@@ -224,6 +227,23 @@ class StepRunner:
         self._found_ids = frozenset()
         self._unequal_shards = False
         self._touched = None
+
+    def _make_adamw(self, options):
+        """codeps_amd.optim.AdamW over the flat groups' parameters (options of cfg.train.optimizer: weight_decay, betas, eps, state_bits,
+        max_grad_norm, skip_nonfinite, seed).  Biases and norm parameters take no weight decay."""
+        from .optim import AdamW
+        named = [(p, g.grad[a:b].view_as(p), None if g.ema is None else g.ema[a:b].view_as(p), gi, pi)
+                 for gi, g in enumerate(self.groups) for pi, (p, a, b) in enumerate(zip(g.params, g.offsets[:-1], g.offsets[1:]))]
+        named = [t for t in named if t[0].dim() > 1] + [t for t in named if t[0].dim() <= 1]
+        decayed = sum(t[0].dim() > 1 for t in named)
+        self._adamw_grads = [t[1] for t in named]
+        self._adamw_place = [(t[3], t[4]) for t in named]          # (group, parameter) of every entry, for the parameters a step does not reach
+        groups = [{"params": [t[0] for t in part], "weight_decay": wd}
+                  for part, wd in ((named[:decayed], float(options.get("weight_decay", 1e-2))), (named[decayed:], 0.0)) if part]
+        return AdamW(groups, lr=self.lr, betas=tuple(options.get("betas", (0.9, 0.999))), eps=float(options.get("eps", 1e-8)),
+                     state_bits=int(options.get("state_bits", 32)), ema=[t[2] for t in named], ema_alpha=self.ema_alpha,
+                     max_norm=options.get("max_grad_norm", None), skip_nonfinite=bool(options.get("skip_nonfinite", False)),
+                     seed=int(options.get("seed", 0)))
 
     def set_key_counts(self, items, rank):
         """Batch-sharded step whose ranks hold DIFFERENT numbers of items per key (ranks
@@ -359,10 +379,19 @@ class StepRunner:
 
     def optimizer_step(self, apply_ema=True):
         """ONE all-reduce of the step's flat gradient buffer, then the fused Adam kernel per flat group (EMA'd modules / the
-        rest).  apply_ema False leaves the EMA copy alone: the reference filters the teacher once per FRAME, after its
+        rest), or AdamW over all of them.  apply_ema False leaves the EMA copy alone: the reference filters the teacher once per FRAME, after its
         `nof_adaptation_steps` optimizer steps (scripts/adapt_codeps.py:266-299)."""
         self.step_count += 1
         self.allreduce_gradients()
+        if self.adamw is not None:
+            grads = self._adamw_grads
+            if self._touched is not None:
+                grads = [g if self._touched[gi] is None or self._touched[gi][pi] else None for g, (gi, pi) in zip(grads, self._adamw_place)]
+            for group in self.adamw.param_groups:
+                if not torch.is_tensor(group["lr"]):
+                    group["lr"] = self.lr
+            self.adamw.step(grads, grad_scale=1.0 / self.world, apply_ema=apply_ema)
+            return
         for i, g in enumerate(self.groups):
             g.adam(None if self._touched is None else self._touched[i], self.lr, 1.0 / self.world, self.ema_alpha, apply_ema)
 

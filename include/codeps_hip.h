@@ -483,6 +483,92 @@ int codeps_adam_ema_step(float* params, const float* grads, float* exp_avg, floa
                          float* ema_params, long long n, int step, float lr, float beta1, float beta2,
                          float eps, float grad_scale, float ema_alpha, codeps_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Norms over the channels of a row (a pixel of an NHWC map, a token): before a block, and at its end fused with gate, residual scale and the next
+ * block's norm.  (No reference counterpart: an alternative to train-mode BatchNorm2d whose statistics do not depend on the batch.)
+ *   full = 0:  h = n(x) w + b
+ *   full = 1:  a = n(x) w + b  (kind NONE: x w + b),  y = residual + scale act(gate) a,  h = n'(y) w' + b'  (next_kind != NONE)
+ *   n(v) = (v - mean v) / sqrt(var v + eps)  (LAYER)   |   v / sqrt(mean v^2 + eps)  (RMS)
+ * x, h and dh have x_type; residual, y and dy res_type (x_type or F32); weight / bias, next_weight / next_bias and gate types of their own.  Every
+ * vector is optional (NULL: weight 1, bias 0, residual 0).  gate: CHANNEL [channels], ITEM [rows / rows_per_item] rows, ELEMENT [rows] rows.
+ * Pitches are elements from row to row (>= channels; rows may start at any element); outputs are dense.  Arithmetic fp32, one rounding per output.
+ * stats (NULL in inference): [rows][4] floats (full = 0: [rows][2]), 16-byte aligned, handed unchanged to _bwd.
+ * _bwd: dy / dh NULL = no gradient of that output (full = 1 needs one of them; with next_kind, dh).  Every gradient pointer may be NULL.  Gradients of
+ * vectors are sums over rows in a fixed order, in the vector's type; the CODEPS_ACC_* bits add them to fp32 contents instead of storing them.
+ * rows = 0 stores zeros into the vectors' gradients (an ITEM gate's is not touched: 0 rows do not tell its size).  No output may overlap an input. */
+#define CODEPS_F32 0
+#define CODEPS_BF16 1
+#define CODEPS_F16 2
+#define CODEPS_NORM_NONE 0
+#define CODEPS_NORM_LAYER 1
+#define CODEPS_NORM_RMS 2
+#define CODEPS_GATE_NONE 0
+#define CODEPS_GATE_CHANNEL 1
+#define CODEPS_GATE_ITEM 2
+#define CODEPS_GATE_ELEMENT 3
+#define CODEPS_GATE_LINEAR 0
+#define CODEPS_GATE_SIGMOID 1
+#define CODEPS_GATE_SILU 2
+#define CODEPS_ACC_WEIGHT 1
+#define CODEPS_ACC_BIAS 2
+#define CODEPS_ACC_NEXT_WEIGHT 4
+#define CODEPS_ACC_NEXT_BIAS 8
+typedef struct {
+    int64_t rows, x_pitch, res_pitch, gate_pitch, dy_pitch, dh_pitch;
+    int32_t channels, rows_per_item, full, kind, next_kind, gate_mode, gate_act;
+    int32_t x_type, res_type, weight_type, gate_type, next_weight_type;
+    float scale, eps, next_eps;
+} codeps_channel_norm_desc;
+int codeps_channel_norm_fwd(const codeps_channel_norm_desc* d, const void* x, const void* residual, const void* gate,
+                            const void* weight, const void* bias, const void* next_weight, const void* next_bias, void* y, void* h,
+                            float* stats, codeps_stream_t stream);
+size_t codeps_channel_norm_bwd_workspace_bytes(const codeps_channel_norm_desc* d);
+int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const void* x, const void* residual, const void* gate,
+                            const void* weight, const void* bias, const void* next_weight, const float* stats, const void* dy,
+                            const void* dh, void* dx, void* dresidual, void* dgate, void* dweight, void* dbias, void* dnext_weight,
+                            void* dnext_bias, int accumulate, void* workspace, size_t workspace_bytes, codeps_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * AdamW over many tensors at once (decoupled weight decay), beside codeps_adam_ema_step on flat buffers:
+ *   g' = g grad_scale c,  c = min(1, max_norm / |grad_scale g|_2) over all tensors (max_norm <= 0: 1)
+ *   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+ *   ema = ema_alpha ema + (1 - ema_alpha) p;   copy = p rounded to bf16 / fp16
+ * Parameters, EMA fp32; gradients fp32, bf16 or fp16.  t is the tensor's own count of steps (device int64, advanced here), so that a captured step
+ * replays as the next one.  A tensor whose gradient pointer is NULL keeps parameter, states and count; its EMA still follows.  ema_alpha < 0: no EMA.
+ * States: bits = 32: exp_avg / exp_avg_sq fp32 at `state_offset` elements.  bits = 8: blocks of 256 elements of one tensor (the last one padded with
+ * zeros), `state_offset` a multiple of 256: m as sign / 4 exponent / 3 mantissa bits, sqrt(v) as 4 exponent / 4 mantissa bits, each block with one
+ * biased exponent byte: value = (-1)^s f 2^(byte - 127), f = mantissa 2^(-14 - mant_bits) for exponent field 0, else (1 + mantissa 2^-mant_bits)
+ * 2^(field - 15); the block's exponent is the smallest under which its largest magnitude fits; byte 0: zeros (nothing of 2^-126 or more), byte 255:
+ * not finite (decodes as NaN).  Codes are rounded to one of the two neighbours with the odds of the place between them, by 16 random bits of
+ * (seed, tensor's index, t, element): rounding to nearest would lose an average's steps, which are far below half a code.  The parameter's update uses
+ * m and v before they are rounded.
+ * Usage: host buffer of n * codeps_adamw_item_bytes(), one codeps_adamw_item_fill per tensor in order (returns the tensor's number of chunks, negative
+ * on error; chunk0 = the sum so far), copied to the device as `items`; chunk_items [n_chunks] int32 = the item of every chunk.
+ * grads, grad_types, chunk0 [n + 1] and groups are HOST arrays, read during the call.
+ * norm (device, nullable): |grad_scale g|_2 of this step is stored there.  skip_nonfinite: a step whose norm is not finite changes nothing. */
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_device;      /* DEVICE scalar that replaces lr, or NULL */
+} codeps_adamw_group;
+size_t codeps_adamw_item_bytes(void);
+long long codeps_adamw_item_fill(void* item, float* param, float* ema, void* copy, int copy_type, long long numel, int bits,
+                                 long long state_offset, long long packed_offset, int group, long long chunk0);
+size_t codeps_adamw_workspace_bytes(int n_items);
+int codeps_adamw_step(const void* items, int n_items, const int* chunk_items, const long long* chunk0, const void* const* grads,
+                      const unsigned char* grad_types, const long long* numels, const codeps_adamw_group* groups, int n_groups,
+                      long long* steps, float* exp_avg, float* exp_avg_sq, unsigned char* exp_avg_codes, unsigned char* exp_avg_exponents,
+                      unsigned char* root_codes, unsigned char* root_exponents, double grad_scale, double max_norm, int skip_nonfinite,
+                      float* norm, unsigned long long seed, double ema_alpha, void* workspace, size_t workspace_bytes,
+                      codeps_stream_t stream);
+/* The values the 8-bit states stand for (exact in bf16), tensors packed without padding at their packed_offset: m and sqrt(v). */
+int codeps_adamw_moments_8bit(const void* items, int n_items, const int* chunk_items, long long n_chunks,
+                              const unsigned char* exp_avg_codes, const unsigned char* exp_avg_exponents, const unsigned char* root_codes,
+                              const unsigned char* root_exponents, void* exp_avg_bf16, void* root_bf16, codeps_stream_t stream);
+/* |scale g|_2 over n tensors (HOST arrays of pointers, types, element counts) -> norm [1] (device), summed in 64 bits in a fixed order. */
+size_t codeps_grad_norm_workspace_bytes(int n_tensors);
+int codeps_grad_norm(const void* const* grads, const unsigned char* grad_types, const long long* numels, int n_tensors, double scale,
+                     float* norm, void* workspace, size_t workspace_bytes, codeps_stream_t stream);
+
 /* SSIMLoss.__call__ (algos/depth.py:128-155) on its own (the training path evaluates it inside
  * codeps_photometric_*): x, y, out [planes][h][w] (planes = B * C of NCHW tensors); ReflectionPad2d(1),
  * 3x3 mean pooling, out = clamp((1 - n / d) / 2, 0, 1).  _bwd: grad_out [planes][h][w] -> grad_x,

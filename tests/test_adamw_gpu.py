@@ -1,0 +1,436 @@
+"""codeps_amd.optim.AdamW and functional.grad_norm against a plain implementation in 64 bits on the CPU.
+
+Tolerances (fixed before the first run).  32-bit states: a moment is two products and a sum, off by at most 3 roundings (3 * 2^-24 of the larger term) per
+step, and errors of earlier steps only decay: 8 * 2^-24 * (|b1 m| + |(1 - b1) g'|) per step, twice that for v (g' is squared).  The parameter adds its own
+rounding and lr * 32 * 2^-24 of the ratio, whose error is that of m, sqrt(v), a reciprocal and two scalars; m may cancel, so its error counts relative to
+its terms.  8-bit states: codes and exponents are EQUAL to those of the 64-bit formula (the kernel decides in 64 bits where fp32 could be wrong)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from codeps_amd import functional as F
+from codeps_amd._lib import CodepsHipError
+from codeps_amd.optim import AdamW
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -24
+MASK = (1 << 64) - 1
+
+
+# ------------------------------------------------------------------------------------------------ the 8-bit format, element by element in 64 bits
+def grid(mant):
+    return [k * 2.0 ** (-14 - mant) for k in range(1 << mant)] + [(1 + k / (1 << mant)) * 2.0 ** e for e in range(-14, 1) for k in range(1 << mant)]
+
+
+def random_bits(seed, tensor, step, n):
+    z = (seed + step * 0x9E3779B97F4A7C15 + tensor * 0xD1B54A32D192ED03) & MASK
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & MASK
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & MASK
+    z ^= z >> 31
+    x = (np.arange(n, dtype=np.uint64) + np.uint64(z & 0xFFFFFFFF)) & np.uint64(0xFFFFFFFF)
+    low = np.uint64(0xFFFFFFFF)
+    x = ((x ^ (x >> np.uint64(16))) * np.uint64(0x7FEB352D)) & low
+    x = x ^ (x >> np.uint64(15)) ^ np.uint64(z >> 32)
+    x = (x * np.uint64(0x846CA68B)) & low
+    x = x ^ (x >> np.uint64(16))
+    return (x & np.uint64(0xFFFF)).astype(np.float64), (x >> np.uint64(16)).astype(np.float64)
+
+
+def encode(x, rho, mant, signed):
+    """x [n] float64 -> (codes padded to whole blocks, exponent bytes, values)."""
+    g = np.array(grid(mant) + [2.0])
+    n, k = len(x), -(-len(x) // 256)
+    codes, exps, vals = np.zeros(k * 256, np.uint8), np.zeros(k, np.uint8), np.zeros(n)
+    for b in range(k):
+        v = x[256 * b:256 * (b + 1)]
+        if not np.isfinite(v).all():
+            exps[b] = 255
+            vals[256 * b:256 * b + len(v)] = np.nan
+            continue
+        top = np.abs(v).max()
+        e = -126
+        while e < 128 and top > g[-2] * 2.0 ** e:
+            e += 1
+        if top < 2.0 ** -126:
+            continue
+        t = np.abs(v) / 2.0 ** e
+        lo = np.searchsorted(g, t, side="right") - 1
+        up = (t - g[lo]) / (g[lo + 1] - g[lo]) + rho[256 * b:256 * b + len(v)] / 65536.0 >= 1.0
+        c = lo + up
+        codes[256 * b:256 * b + len(v)] = c + (128 * (v < 0) if signed else 0)
+        exps[b] = e + 127
+        vals[256 * b:256 * b + len(v)] = np.where(v < 0, -1, 1) * g[c] * 2.0 ** e
+    return codes, exps, vals
+
+
+class Plain:
+    """The same optimizer in 64 bits on the CPU, with a bound of the fp32 kernel's error beside every value."""
+
+    def __init__(self, params, decays, bits, lr, betas, eps, max_norm=None, ema=None, ema_alpha=0.99, seed=0):
+        self.p = [p.detach().double().cpu().numpy().reshape(-1).copy() for p in params]
+        self.m, self.v = [np.zeros_like(p) for p in self.p], [np.zeros_like(p) for p in self.p]
+        self.pe, self.me, self.ve = ([np.zeros_like(p) for p in self.p] for _ in range(3))
+        self.steps = [0] * len(self.p)
+        self.decays, self.bits, self.lr, self.betas, self.eps, self.max_norm, self.seed = decays, bits, lr, betas, eps, max_norm, seed
+        self.ema = None if ema is None else [None if e is None else e.detach().double().cpu().numpy().reshape(-1).copy() for e in ema]
+        self.ema_alpha, self.stored = ema_alpha, {}
+
+    def step(self, grads, grad_scale=1.0, lr=None, apply_ema=True):
+        lr = self.lr if lr is None else lr
+        b1, b2 = self.betas
+        gs = [None if g is None else g.double().cpu().numpy().reshape(-1) for g in grads]
+        self.norm = abs(grad_scale) * math.sqrt(sum(float((g ** 2).sum()) for g in gs if g is not None))
+        c = grad_scale * (self.max_norm / self.norm if self.max_norm and self.norm > self.max_norm else 1.0)
+        for i, g in enumerate(gs):
+            if g is not None:
+                g = g * c
+                self.steps[i] += 1
+                t = self.steps[i]
+                ms, vs = np.abs(b1 * self.m[i]) + np.abs((1 - b1) * g), b2 * self.v[i] + (1 - b2) * g * g
+                self.me[i] = b1 * self.me[i] + 8 * U * ms
+                self.ve[i] = b2 * self.ve[i] + 16 * U * vs
+                self.m[i] = b1 * self.m[i] + (1 - b1) * g
+                self.v[i] = vs
+                den = np.sqrt(self.v[i] / (1 - b2 ** t)) + self.eps
+                rate = lr / (1 - b1 ** t)
+                with np.errstate(invalid="ignore"):
+                    rel_v = np.where(self.v[i] > 0, self.ve[i] / np.maximum(self.v[i], 1e-300), 0.0)
+                    self.pe[i] += 2 * U * np.abs(self.p[i]) + np.abs(rate) * (self.me[i] + ms * (rel_v + 32 * U)) / den
+                    self.p[i] = self.p[i] * (1 - lr * self.decays[i]) - rate * self.m[i] / den
+                if self.bits[i] == 8:
+                    rm, rr = random_bits(self.seed, i, t, len(g))
+                    cm, em, self.m[i] = encode(self.m[i], rm, 3, True)
+                    cr, er, root = encode(np.sqrt(self.v[i]), rr, 4, False)
+                    self.v[i] = root ** 2
+                    self.me[i][:] = self.ve[i][:] = 0
+                    self.stored[i] = (cm, em, cr, er)
+            if self.ema is not None and apply_ema and self.ema[i] is not None:
+                self.ema[i] = self.ema_alpha * self.ema[i] + (1 - self.ema_alpha) * self.p[i]
+
+
+def check(opt, plain, copies=None):
+    flat = lambda t: t.detach().double().cpu().numpy().reshape(-1)                                # noqa: E731
+    assert opt.steps.tolist() == plain.steps
+    for i, p in enumerate(opt.params):
+        off, n = opt._offsets[i], p.numel()
+        err = np.abs(flat(p) - plain.p[i])
+        assert (err <= plain.pe[i] + 2 * U * np.abs(plain.p[i])).all(), ("p", i, float((err / (plain.pe[i] + 1e-300)).max()))
+        if plain.bits[i] == 32:
+            for have, want, bar in ((opt.exp_avg, plain.m[i], plain.me[i]), (opt.exp_avg_sq, plain.v[i], plain.ve[i])):
+                assert (np.abs(flat(have[off:off + n]) - want) <= bar + 1e-44).all(), ("moments", i)
+        elif i in plain.stored:
+            k = -(-n // 256)
+            cm, em, cr, er = plain.stored[i]
+            assert np.array_equal(opt.exp_avg_exponents[off // 256:off // 256 + k].cpu().numpy(), em), ("exponents of m", i)
+            assert np.array_equal(opt.root_exponents[off // 256:off // 256 + k].cpu().numpy(), er), ("exponents of the root", i)
+            assert np.array_equal(opt.exp_avg_codes[off:off + 256 * k].cpu().numpy(), cm), ("codes of m", i)
+            assert np.array_equal(opt.root_codes[off:off + 256 * k].cpu().numpy(), cr), ("codes of the root", i)
+        if plain.ema is not None and plain.ema[i] is not None:
+            err = np.abs(flat(opt._ema[i]) - plain.ema[i])
+            assert (err <= 8 * (plain.pe[i] + U * np.abs(plain.ema[i]) + U * np.abs(plain.p[i]))).all(), ("ema", i)
+        if opt._copies[i] is not None and copies:
+            assert torch.equal(opt._copies[i], p.detach().to(opt._copies[i].dtype)), ("copy", i)
+
+
+def tensors(sizes, seed, spread=1e-2):
+    g = torch.Generator().manual_seed(seed)
+    return [(spread * torch.randn(*(s if isinstance(s, tuple) else (s,)), generator=g)).to(DEV) for s in sizes]
+
+
+def gradients(params, seed, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    return [(1e-3 * torch.randn(p.shape, generator=g) * torch.exp(2 * torch.randn(p.shape, generator=g))).to(dtype).to(DEV) for p in params]
+
+
+SIZES = [1, 2, 3, 5, 255, 256, 257, (16, 16, 3, 3), 2047, 2048, 2049, (64, 100), 4099, 10001, (0,)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_steps_against_64_bits(bits, dtype):
+    """Every size around a chunk and a block; decay by group, EMA, copies, clipping, a scale, tensors without a gradient."""
+    params = tensors(SIZES, 1, 0.05)
+    ema = [p + 0.01 if i % 3 == 0 else None for i, p in enumerate(params)]
+    copies = [torch.zeros_like(p, dtype=BF16 if i % 2 else F16) if i % 4 else None for i, p in enumerate(params)]
+    mats = [i for i, p in enumerate(params) if i % 2 == 0]
+    order = mats + [i for i in range(len(params)) if i % 2]
+    params, ema, copies = ([v[i] for i in order] for v in (params, ema, copies))
+    opt = AdamW([{"params": params[:len(mats)], "weight_decay": 0.1}, {"params": params[len(mats):], "weight_decay": 0.0, "lr": 3e-3}], lr=3e-3, betas=(0.9, 0.99),
+                state_bits=bits, small_numel=256, ema=ema, ema_alpha=0.9, copies=copies, max_norm=0.05, seed=77)
+    held = [bits if p.numel() >= 256 else 32 for p in params]
+    plain = Plain(params, [0.1] * len(mats) + [0.0] * (len(params) - len(mats)), held, 3e-3, (0.9, 0.99), 1e-8, 0.05, ema, 0.9, 77)
+    for k in range(4):
+        grads = gradients(params, 100 + k, dtype)
+        if k == 2:
+            grads = [None if i % 3 == 1 else g for i, g in enumerate(grads)]
+        opt.step(grads, grad_scale=0.5, apply_ema=k != 1)
+        plain.step(grads, 0.5, apply_ema=k != 1)
+        check(opt, plain, copies=k == 0)
+        assert abs(float(opt.grad_norm) - plain.norm) <= 2 * U * plain.norm
+
+
+def test_default_gradients_mixed_types_and_zero_grad():
+    params = [torch.nn.Parameter(p) for p in tensors([300, (7, 9), 4], 3)]
+    opt = AdamW(params, lr=1e-2, weight_decay=0.0)
+    plain = Plain(params, [0.0] * 3, [32] * 3, 1e-2, (0.9, 0.999), 1e-8)
+    params[0].grad = gradients(params, 5)[0]
+    params[2].grad = gradients(params, 6)[2]
+    opt.step()
+    plain.step([params[0].grad, None, params[2].grad])
+    check(opt, plain)
+    opt.zero_grad(set_to_none=False)
+    assert not params[0].grad.any() and params[1].grad is None
+    opt.zero_grad()
+    before = [p.detach().clone() for p in params]
+    opt.step()                                                       # nothing has a gradient: nothing moves
+    assert all(torch.equal(a, b) for a, b in zip(before, params)) and opt.steps.tolist() == [1, 0, 1]
+    grads = [g.to(t) for g, t in zip(gradients(params, 8), (F16, F32, BF16))]
+    opt.step(grads)
+    plain.step(grads)
+    check(opt, plain)
+
+
+def test_more_tensors_than_one_launch_takes_and_unaligned_views():
+    """331 + 331 tensors as views of flat buffers (starts at any multiple of an element), 32 and 8 bits mixed by size."""
+    g = torch.Generator().manual_seed(2)
+    sizes = torch.randint(1, 700, (662,), generator=g).tolist()
+    flat = 0.1 * torch.randn(sum(sizes) + 1, generator=g)
+    flat, grad = flat.to(DEV), (1e-2 * torch.randn(sum(sizes) + 1, generator=g)).to(BF16).to(DEV)
+    cut = lambda t: list(t[1:].split(sizes))                                                      # noqa: E731
+    params, grads = cut(flat), cut(grad)
+    opt = AdamW(params, lr=1e-3, state_bits=8, small_numel=300, max_norm=1.0, seed=5)
+    plain = Plain(params, [0.01] * 662, [8 if n >= 300 else 32 for n in sizes], 1e-3, (0.9, 0.999), 1e-8, 1.0, seed=5)
+    for _ in range(2):
+        opt.step(grads)
+        plain.step(grads)
+        check(opt, plain)
+    first = float(flat[0])
+    assert first == float(flat[0])                                   # (the element in front of the views)
+    m, r = opt.moments_8bit()
+    big = [i for i, n in enumerate(sizes) if n >= 300]
+    assert np.array_equal(m.double().cpu().numpy(), np.concatenate([plain.m[i] for i in big]))
+    assert np.array_equal(r.double().cpu().numpy() ** 2, np.concatenate([plain.v[i] for i in big]))
+
+
+def test_layouts():
+    p = torch.randn(8, 6, 5, 5, device=DEV).contiguous(memory_format=torch.channels_last)
+    q = p.detach().clone().contiguous()
+    g = torch.randn(8, 6, 5, 5, device=DEV)
+    a, b = AdamW([p], lr=1e-2), AdamW([q], lr=1e-2)
+    for _ in range(2):
+        a.step([g])                                                  # gradient in another layout than its parameter
+        b.step([g])
+        b.step([g.contiguous(memory_format=torch.channels_last)])
+        a.step([g.contiguous(memory_format=torch.channels_last)])
+    assert torch.equal(p, q)
+    q.data = q.data.clone()                                          # moved: the table follows
+    p2 = p.detach().clone()
+    a.step([g])
+    b.step([g])
+    assert torch.equal(p, q) and not torch.equal(p, p2)
+
+
+def test_eight_bit_rounding_is_unbiased_and_averages_decay():
+    """65536 elements of one value: the mean of what is stored is the value (4 standard errors); with zero gradients the stored moments fall with b^t, which
+    rounding to the nearest code would keep from happening (0.1 % of a value is far below half a code)."""
+    n, lr = 65536, 0.0
+    p = torch.zeros(n, device=DEV)
+    opt = AdamW([p], lr=lr, betas=(0.5, 0.999), state_bits=8, seed=3)
+    g = torch.full((n,), 1.37e-3, device=DEV)
+    g[::256] = 5e-3                                                  # (the block's largest value, so that the others are not at its top)
+    opt.step([g])
+    m, r = (t.double() for t in opt.moments_8bit())
+    rest = torch.ones(n, dtype=torch.bool, device=DEV)
+    rest[::256] = False
+    for have, want in ((m[rest].mean(), 0.5 * 1.37e-3), (r[rest].mean(), math.sqrt(0.001) * 1.37e-3)):
+        assert abs(float(have) / want - 1) <= 4 * 0.125 / 2 / math.sqrt(n)
+    zero = torch.zeros_like(g)
+    for _ in range(700):
+        opt.step([zero])
+    m, r = (t.double() for t in opt.moments_8bit())
+    # the root's mean falls with sqrt(b2)^700 = 0.704 (its square is updated: a step's rounding noise, at most (2^-5)^2 / 4 of the square, pulls the mean of
+    # the root up by about that share of b2's decay: the bound allows 0.72 to 0.99 of the value before, nearest rounding would leave 1.0)
+    left = float(r[rest].mean()) / (math.sqrt(0.001) * 1.37e-3)
+    assert 0.5 < left < 0.99, left
+    assert float(m.abs().max()) == 0.0                               # 0.5^700
+
+
+def test_non_finite_gradients():
+    params = tensors([1000, 5000], 1)
+    grads = gradients(params, 2)
+    grads[1][4321] = float("inf")
+    opt = AdamW(params, state_bits=8, small_numel=2000, max_norm=1.0, skip_nonfinite=True, ema=[p.clone() for p in params])
+    keep = [p.clone() for p in params] + [e.clone() for e in opt._ema]
+    opt.step(grads)
+    assert all(torch.equal(a, b) for a, b in zip(keep, params + opt._ema)) and opt.steps.tolist() == [0, 0] and math.isinf(float(opt.grad_norm))
+    assert not opt.exp_avg.any() and not opt.exp_avg_codes.any()
+    opt.skip_nonfinite, opt.max_norm = False, None
+    grads[1][4321] = float("nan")
+    opt.step(grads)
+    m, r = opt.moments_8bit()
+    bad = torch.arange(5000, device=DEV) // 256 == 4321 // 256       # the block of the NaN, and nothing beside it
+    assert torch.isnan(m[bad]).all() and torch.isnan(r[bad]).all() and torch.isfinite(m[~bad]).all() and torch.isfinite(r[~bad]).all()
+    assert torch.isnan(params[1]).sum() == 1 and torch.isfinite(params[0]).all()
+
+
+def test_tiny_and_huge_moments():
+    """Blocks near both ends of fp32: zeros below 2^-126, NaN where the block's unit would be 2^128; values in between keep their bits."""
+    p = tensors([1024], 1)[0]
+    g = torch.zeros(1024)
+    g[0], g[256], g[512], g[768] = 1e-39, 1e-30, 1.0, 3.4e38
+    opt = AdamW([p], lr=0.0, betas=(0.0, 0.0), state_bits=8, small_numel=1, weight_decay=0.0)
+    opt.step([g.to(DEV)])
+    assert opt.exp_avg_exponents.tolist() == [0, 127 - 100, 127, 255]
+    m = opt.moments_8bit()[0].float().cpu()
+    assert float(m[0]) == 0.0 and abs(float(m[256]) / 1e-30 - 1) <= 0.125 and float(m[512]) == 1.0 and torch.isnan(m[768:]).all() and not m[1:256].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_replays_as_the_next_step(bits):
+    """Capture with a learning rate on the device; every replay equals the eager step bit for bit (step counts, random bits and clipping are on the device)."""
+    lr = torch.tensor(1e-2, device=DEV)
+    mine, theirs = tensors([5000, 300, 9000], 4), tensors([5000, 300, 9000], 4)
+    grads = gradients(mine, 1)
+    a = AdamW(mine, lr=lr, state_bits=bits, max_norm=0.1, seed=9, ema=[p.clone() for p in mine])
+    b = AdamW(theirs, lr=1e-2, state_bits=bits, max_norm=0.1, seed=9, ema=[p.clone() for p in theirs])
+    a.step(grads)
+    b.step(grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(grads)
+    for k in range(4):
+        fresh = gradients(mine, 10 + k)
+        for g, f in zip(grads, fresh):
+            g.copy_(f)
+        rate = float(np.float32(1e-2 / (k + 1)))
+        lr.fill_(rate)
+        b.param_groups[0]["lr"] = rate
+        graph.replay()
+        b.step(fresh)
+        torch.cuda.synchronize()
+        for x, y in zip(mine + a._ema, theirs + b._ema):
+            assert torch.equal(x, y), k
+        sa, sb = a.state_dict(), b.state_dict()
+        assert all(torch.equal(sa[n], sb[n]) for n in sa if n != "param_groups") and float(a.grad_norm) == float(b.grad_norm)
+
+
+def test_state_dict_continues_the_run():
+    a_p = tensors([6000, 50], 2)
+    a = AdamW(a_p, lr=1e-2, state_bits=8, seed=1)
+    for k in range(3):
+        a.step(gradients(a_p, k))
+    b_p = [p.clone() for p in a_p]
+    b = AdamW(b_p, lr=5.0, state_bits=8, seed=1)
+    b.load_state_dict(a.state_dict())
+    for k in range(3, 5):
+        a.step(gradients(a_p, k))
+        b.step(gradients(b_p, k))
+    assert all(torch.equal(x, y) for x, y in zip(a_p, b_p)) and b.param_groups[0]["lr"] == 1e-2
+    for other in (AdamW([p.clone() for p in a_p], state_bits=32), AdamW(tensors([6000], 2), state_bits=8)):
+        with pytest.raises(CodepsHipError):
+            other.load_state_dict(a.state_dict())
+
+
+def test_updates_are_seen_by_autograd_and_by_the_weight_packs():
+    w = torch.nn.Parameter(torch.randn(16, 16, 1, 1, device=DEV))
+    x = torch.randn(1, 8, 8, 16, device=DEV)
+    opt = AdamW([w], lr=0.5, weight_decay=0.0)
+    (w * w).sum().backward()
+    held = (w * w).sum()                                             # its backward would need the weight from before the step
+    y0 = F.conv2d(x, w).detach()
+    opt.step()
+    with pytest.raises(RuntimeError):
+        held.backward()
+    y1 = F.conv2d(x, w).detach()
+    want = torch.einsum("bhwc,oc->bhwo", x.double().cpu(), w.detach().double().cpu()[:, :, 0, 0])
+    assert not torch.equal(y0, y1) and float((y1.double().cpu() - want).abs().max()) <= 1e-4
+
+
+def test_elements_beyond_32_bit_offsets():
+    """One tensor of 2^31 + 300 elements with 8-bit states: its last elements are updated, and stored, as the formula says."""
+    n = (1 << 31) + 300
+    p, g = torch.zeros(n, device=DEV), torch.zeros(n, dtype=BF16, device=DEV)
+    tail = gradients([torch.zeros(600)], 3, BF16)[0]
+    g[-600:] = tail
+    opt = AdamW([p], lr=1e-2, state_bits=8, seed=12, max_norm=1e-3)
+    opt.step([g])
+    norm = float(tail.double().norm())
+    assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm and abs(float(F.grad_norm([g])) - norm) <= 2 * U * norm
+    scaled = tail.double().cpu().numpy() * min(1.0, 1e-3 / norm)
+    want = -1e-2 * scaled / (np.abs(scaled) + 1e-8)
+    assert np.abs(p[-600:].double().cpu().numpy() - want).max() <= 1e-2 * 64 * U
+    assert not p[:1 << 20].any() and not p[(1 << 31) - 1000:(1 << 31) - 300].any()
+    z = 0.1 * scaled
+    blocks = opt.exp_avg_codes[-512:].cpu().numpy()                   # the last whole block and the padded one: 300 = 256 + 44 elements behind 2^31
+    i = np.arange(1 << 31, n, dtype=np.uint64)
+    seed = (12 + 0x9E3779B97F4A7C15) & MASK
+    seed = ((seed ^ (seed >> 30)) * 0xBF58476D1CE4E5B9) & MASK
+    seed = ((seed ^ (seed >> 27)) * 0x94D049BB133111EB) & MASK
+    seed ^= seed >> 31
+    low = np.uint64(0xFFFFFFFF)
+    x = (i + np.uint64(seed & 0xFFFFFFFF)) & low
+    x = ((x ^ (x >> np.uint64(16))) * np.uint64(0x7FEB352D)) & low
+    x = ((x ^ (x >> np.uint64(15)) ^ np.uint64(seed >> 32)) * np.uint64(0x846CA68B)) & low
+    x ^= x >> np.uint64(16)
+    codes, _, _ = encode(z[-300:], (x & np.uint64(0xFFFF)).astype(np.float64), 3, True)
+    assert np.array_equal(blocks, codes)
+
+
+# ------------------------------------------------------------------------------------------------------------------------ gradient norm
+def test_grad_norm():
+    g = torch.Generator().manual_seed(7)
+    sizes = [1, 3, 4095, 4096, 4097, 100000] + torch.randint(1, 3000, (400,), generator=g).tolist()
+    ts = [(torch.randn(n, generator=g) * 10.0 ** (i % 4)).to((F32, BF16, F16)[i % 3]).to(DEV) for i, n in enumerate(sizes)]
+    ts.insert(5, torch.zeros(0, device=DEV))
+    ts.insert(0, torch.zeros(0, device=DEV))
+    want = math.sqrt(sum(float(t.double().square().sum()) for t in ts))
+    got = F.grad_norm([None] + ts + [None], scale=-0.25)
+    assert got.shape == () and got.dtype == F32 and abs(float(got) - 0.25 * want) <= 2 * U * want
+    assert float(F.grad_norm(ts)) == float(F.grad_norm(ts))
+    strided = torch.randn(50, 70, device=DEV)[:, ::2]
+    assert abs(float(F.grad_norm([strided])) - float(strided.double().norm())) <= 2 * U * float(strided.double().norm())
+    assert abs(float(F.grad_norm([torch.full((1000,), 1e30, device=DEV)])) / (1e30 * math.sqrt(1000)) - 1) <= 2 * U
+    assert math.isinf(float(F.grad_norm([torch.tensor([1.0, float("-inf")], device=DEV)]))) and math.isnan(float(F.grad_norm([torch.tensor([float("nan")], device=DEV)])))
+    assert float(F.grad_norm([torch.zeros(0, device=DEV)])) == 0.0
+
+
+def test_grad_norm_in_a_graph():
+    ts = gradients([torch.zeros(5000), torch.zeros(70)], 1)
+    F.grad_norm(ts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.grad_norm(ts)
+    for k in range(3):
+        for t, f in zip(ts, gradients(ts, 50 + k)):
+            t.copy_(f)
+        want = float(F.grad_norm(ts))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float(out) == want
+
+
+def test_refusals():
+    p = torch.zeros(10, device=DEV)
+    for bad in (lambda: AdamW([]), lambda: AdamW([{"params": []}]), lambda: AdamW([p.half()]), lambda: AdamW([p, p]), lambda: AdamW([torch.zeros(4, 6, device=DEV)[:, ::2]]),
+                lambda: AdamW([p], state_bits=16), lambda: AdamW([p], max_norm=0.0), lambda: AdamW([p], ema=[p.half()]), lambda: AdamW([p], ema=[]),
+                lambda: AdamW([p], copies=[p.clone()]), lambda: AdamW([p], copies=[torch.zeros(9, dtype=BF16, device=DEV)]), lambda: AdamW([{"params": [p], "momentum": 1}]),
+                lambda: AdamW([{"params": [torch.zeros(1, device=DEV)]} for _ in range(17)]), lambda: F.grad_norm([]), lambda: F.grad_norm([None]),
+                lambda: F.grad_norm([p.double()]), lambda: F.grad_norm([p, p.cpu()])):
+        with pytest.raises(CodepsHipError):
+            bad()
+    opt = AdamW([p, torch.zeros(3, 4, device=DEV)])
+    for grads in ([p], [p, torch.zeros(4, 3, device=DEV)], [p.cpu(), None], [p.double(), None]):
+        with pytest.raises(CodepsHipError):
+            opt.step(grads)
+    for key, value in (("betas", (1.0, 0.9)), ("betas", (0.9, -0.1)), ("eps", -1.0)):
+        opt = AdamW([p], **{key: value})
+        with pytest.raises(CodepsHipError):
+            opt.step([p])
+    with pytest.raises(CodepsHipError):
+        AdamW([p], lr=torch.zeros(2, device=DEV)).step([p])
+    with pytest.raises(CodepsHipError):
+        AdamW([p]).moments_8bit()
