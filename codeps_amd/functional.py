@@ -3,6 +3,7 @@
 PyTorch supplies device memory (caching allocator), the current HIP stream and the autograd tape;
 all arithmetic happens in libcodeps_hip.so.  Every function raises on CPU tensors -- no fallback.
 """
+import array
 import ctypes
 import os
 import weakref
@@ -2349,19 +2350,28 @@ _GATE_ACTS = {None: 0, "sigmoid": 1, "silu": 2}
 _MAX_NORM_CHANNELS = 8192
 
 
-class _OnDevice:
-    """Makes the tensors' device the current one for the launches inside (nothing to do when it is: torch.cuda.device costs microseconds)."""
+_raw_stream = torch._C._cuda_getCurrentRawStream          # (device index) -> hipStream_t; torch.cuda.current_stream builds an object (4 us)
 
-    def __init__(self, device):
-        self.scope = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.scope is not None:
-            self.scope.__enter__()
+def _on_device(device):
+    """A context that makes `device` the current one for launches, None when it is already (torch.cuda.device costs microseconds)."""
+    return None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
-    def __exit__(self, *exc):
-        if self.scope is not None:
-            self.scope.__exit__(*exc)
+
+def _launch(device, what, call, *args):
+    """check(call(*args, stream)) on the current stream of `device`."""
+    scope = _on_device(device)
+    if scope is None:
+        rc = call(*args, _raw_stream(device.index))
+    else:
+        with scope:
+            rc = call(*args, _raw_stream(device.index))
+    if rc != 0:
+        check(rc, what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _pitched(t):
@@ -2395,89 +2405,101 @@ def _vector(v, c, what, device):
     return v.contiguous()
 
 
+def _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, want_stats):
+    """One forward launch.  cfg = (full, kind, eps, gate mode, gate activation, rows per item, scale, next kind, next eps)."""
+    full, kind, eps, mode, act, per_item, scale, nkind, neps = cfg
+    c = x.shape[-1]
+    rows = x.numel() // c
+    xr, xp = _pitched(x)
+    xt = rt = _TYPES[x.dtype]
+    rr, rp, gr, gp, gt = None, c, None, c, 0
+    if residual is not None:
+        rr, rp = _pitched(residual)
+        rt = _TYPES[residual.dtype]
+    if gate is not None:
+        gr, gp = _pitched(gate)
+        gt = _TYPES[gate.dtype]
+    vec, nvec = weight if weight is not None else bias, next_weight if next_weight is not None else next_bias
+    d = _lib.ChannelNormDesc(rows, xp, rp, gp, c, c, c, per_item, full, kind, nkind, mode, act, xt, rt, 0 if vec is None else _TYPES[vec.dtype], gt,
+                             0 if nvec is None else _TYPES[nvec.dtype], scale, eps, neps)
+    y = (x if residual is None else residual).new_empty(x.shape) if full else None
+    h = x.new_empty(x.shape) if (nkind or not full) else None
+    stats = torch.empty((rows, 4 if full else 2), dtype=torch.float32, device=x.device) if want_stats else None
+    _launch(x.device, "codeps_channel_norm_fwd", lib().codeps_channel_norm_fwd, ctypes.byref(d), xr.data_ptr(), _at(rr), _at(gr), _at(weight), _at(bias),
+            _at(next_weight), _at(next_bias), _at(y), _at(h), _at(stats))
+    return y, h, stats, d, xr, rr, gr
+
+
 class _ChannelNorm(torch.autograd.Function):
-    """Both public forms.  cfg = (full, kind, eps, gate mode, gate activation, rows per item, scale, next kind, next eps)."""
+    """Both public forms with gradients (cfg: _channel_norm_fwd)."""
 
     @staticmethod
     def forward(ctx, x, residual, gate, weight, bias, next_weight, next_bias, cfg):
-        full, kind, eps, mode, act, per_item, scale, nkind, neps = cfg
-        c = x.shape[-1]
-        d = _lib.ChannelNormDesc()
-        d.rows, d.channels, d.rows_per_item, d.full = x.numel() // c, c, per_item, full
-        d.kind, d.next_kind, d.gate_mode, d.gate_act = kind, nkind, mode, act
-        d.x_type = _TYPES[x.dtype]
-        xr, d.x_pitch = _pitched(x)
-        d.res_type, d.res_pitch = d.x_type, c
-        rr = None
-        if residual is not None:
-            rr, d.res_pitch = _pitched(residual)
-            d.res_type = _TYPES[residual.dtype]
-        gr = None
-        if gate is not None:
-            gr, d.gate_pitch = _pitched(gate)
-            d.gate_type = _TYPES[gate.dtype]
-        vec = weight if weight is not None else bias
-        d.weight_type = 0 if vec is None else _TYPES[vec.dtype]
-        vec = next_weight if next_weight is not None else next_bias
-        d.next_weight_type = 0 if vec is None else _TYPES[vec.dtype]
-        d.scale, d.eps, d.next_eps = scale, eps, neps
-        y = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device) if full else None
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if (nkind or not full) else None
-        stats = torch.empty(d.rows, 4 if full else 2, dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
-        with _OnDevice(x.device):
-            check(lib().codeps_channel_norm_fwd(ctypes.byref(d), ptr(xr), ptr(rr), ptr(gr), ptr(weight), ptr(bias), ptr(next_weight), ptr(next_bias),
-                                                ptr(y), ptr(h), ptr(stats), stream_ptr()), "codeps_channel_norm_fwd")
-        if stats is not None:
-            ctx.save_for_backward(xr, rr if nkind else None, gr, weight, bias, next_weight, stats)
-            ctx.d, ctx.gate_shape, ctx.res_dtype = d, None if gate is None else gate.shape, None if residual is None else residual.dtype
-            vectors = (weight, bias, next_weight, next_bias)
-            ctx.vec_dtypes = [None if v is None else v.dtype for v in vectors]
-            ctx.sinks = [grad_sink(v) if v is not None and v.requires_grad else None for v in vectors]     # (flat-gradient views: fp32, contiguous)
+        y, h, stats, d, xr, rr, gr = _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, True)
+        ctx.save_for_backward(xr, rr if d.next_kind else None, gr, weight, bias, next_weight, stats)
+        ctx.d, ctx.gate_shape, ctx.res_dtype = d, None if gate is None else gate.shape, None if residual is None else residual.dtype
+        vectors = (weight, bias, next_weight, next_bias)
+        ctx.vec_dtypes = [None if v is None else v.dtype for v in vectors]
+        ctx.sinks = [grad_sink(v) if v is not None and v.requires_grad else None for v in vectors]     # (flat-gradient views: fp32, contiguous)
         ctx.set_materialize_grads(False)
-        if full:
-            return (y, h) if nkind else y
-        return h
+        if not d.full:
+            return h
+        return (y, h) if d.next_kind else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *douts):
-        x, residual, gate, weight, bias, next_weight, stats = ctx.saved_tensors
-        d0 = ctx.d
-        d = type(d0).from_buffer_copy(d0)             # (two backward passes of one forward may run at once)
-        c, dev, need = d.channels, x.device, ctx.needs_input_grad
-        dy, dh = (douts[0], douts[1] if d.next_kind else None) if d.full else (None, douts[0])
-        if dy is None and dh is None:
-            return (None,) * 8
-        if dy is not None:
-            dy, d.dy_pitch = _pitched(dy)
-        if dh is not None:
-            dh, d.dh_pitch = _pitched(dh)
-        elif d.next_kind:                             # h is not part of the loss: the block's end alone
-            d.next_kind = 0
-            residual = None
-        empty = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)                     # noqa: E731
-        dx = empty(x.shape, x.dtype) if need[0] else None
-        dres = empty(x.shape, ctx.res_dtype) if need[1] else None
-        dgate = (empty if d.rows else lambda s, t: torch.zeros(s, dtype=t, device=dev))(ctx.gate_shape, gate.dtype) if need[2] else None
-        outs, acc = [], 0
-        for i in range(4):
-            out = None
-            if need[3 + i] and (i < 2 or d.next_kind):
-                out = ctx.sinks[i]
-                if out is not None:
-                    acc |= 1 << i
-                else:
-                    out = empty((c,), ctx.vec_dtypes[i])
-            outs.append(out)
-        with _OnDevice(dev):
-            nbytes = lib().codeps_channel_norm_bwd_workspace_bytes(ctypes.byref(d))
-            if nbytes == 0:
-                check(-1, "codeps_channel_norm_bwd_workspace_bytes")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)      # not a cached one: captured graphs must not share it
-            check(lib().codeps_channel_norm_bwd(ctypes.byref(d), ptr(x), ptr(residual), ptr(gate), ptr(weight), ptr(bias), ptr(next_weight), ptr(stats),
-                                                ptr(dy), ptr(dh), ptr(dx), ptr(dres), ptr(dgate), ptr(outs[0]), ptr(outs[1]), ptr(outs[2]), ptr(outs[3]),
-                                                acc, ptr(ws), nbytes, stream_ptr()), "codeps_channel_norm_bwd")
-        return (dx, dres, dgate) + tuple(None if ctx.sinks[i] is not None else outs[i] for i in range(4)) + (None,)
+        if torch.is_grad_enabled():                   # (create_graph: a second derivative raises instead of being silently zero)
+            return _channel_norm_bwd_once(ctx, *douts)
+        return _channel_norm_bwd(ctx, *douts)
+
+
+def _channel_norm_bwd(ctx, *douts):
+    x, residual, gate, weight, bias, next_weight, stats = ctx.saved_tensors
+    d = _lib.ChannelNormDesc.from_buffer_copy(ctx.d)  # (two backward passes of one forward may run at once)
+    c, dev, need, sinks = d.channels, x.device, ctx.needs_input_grad, ctx.sinks
+    dy, dh = (douts[0], douts[1] if d.next_kind else None) if d.full else (None, douts[0])
+    if dy is None and dh is None:
+        return (None,) * 8
+    if dy is not None:
+        dy, d.dy_pitch = _pitched(dy)
+    if dh is not None:
+        dh, d.dh_pitch = _pitched(dh)
+    elif d.next_kind:                                 # h is not part of the loss: the block's end alone
+        d.next_kind = 0
+        residual = None
+    dx = x.new_empty(x.shape) if need[0] else None
+    dres = torch.empty(x.shape, dtype=ctx.res_dtype, device=dev) if need[1] else None
+    dgate = (gate.new_empty if d.rows else gate.new_zeros)(ctx.gate_shape) if need[2] else None
+    outs, acc = [None] * 4, 0
+    for i in range(4 if d.next_kind else 2):
+        if need[3 + i]:
+            if sinks[i] is not None:
+                outs[i], acc = sinks[i], acc | 1 << i
+            else:
+                outs[i] = torch.empty(c, dtype=ctx.vec_dtypes[i], device=dev)
+    nbytes = lib().codeps_channel_norm_bwd_workspace_bytes(ctypes.byref(d))
+    if nbytes == 0:
+        check(-1, "codeps_channel_norm_bwd_workspace_bytes")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)              # not a cached one: captured graphs must not share it
+    _launch(dev, "codeps_channel_norm_bwd", lib().codeps_channel_norm_bwd, ctypes.byref(d), x.data_ptr(), _at(residual), _at(gate), _at(weight), _at(bias),
+            _at(next_weight), stats.data_ptr(), _at(dy), _at(dh), _at(dx), _at(dres), _at(dgate), _at(outs[0]), _at(outs[1]), _at(outs[2]), _at(outs[3]),
+            acc, ws.data_ptr(), nbytes)
+    outs = [None if sinks[i] is not None else outs[i] for i in range(4)]
+    return (dx, dres, dgate, *outs, None)
+
+
+_channel_norm_bwd_once = torch.autograd.function.once_differentiable(_channel_norm_bwd)
+
+
+def _channel_norm_apply(x, residual, gate, weight, bias, next_weight, next_bias, cfg):
+    if torch.is_grad_enabled():
+        for t in (x, residual, gate, weight, bias, next_weight, next_bias):
+            if t is not None and t.requires_grad:
+                return _ChannelNorm.apply(x, residual, gate, weight, bias, next_weight, next_bias, cfg)
+    y, h = _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, False)[:2]
+    if not cfg[0]:
+        return h
+    return (y, h) if cfg[7] else y
 
 
 def _check_rows(x, what):
@@ -2509,7 +2531,7 @@ def channel_norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
     if kind is None:
         raise CodepsHipError("channel_norm: kind is \"layer\" or \"rms\"")
     weight, bias = _check_norm(kind, weight, bias, eps, c, "channel_norm", x.device)
-    return _ChannelNorm.apply(x, None, None, weight, bias, None, None, (0, _NORM_KINDS[kind], eps, 0, 0, 1, 1.0, 0, 0.0))
+    return _channel_norm_apply(x, None, None, weight, bias, None, None, (0, _NORM_KINDS[kind], eps, 0, 0, 1, 1.0, 0, 0.0))
 
 
 def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=None, gate_act=None, scale=1.0, next_kind=None,
@@ -2544,8 +2566,8 @@ def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="lay
             mode, per_item = 2, max(1, x.numel() // c // max(1, x.shape[0]))
         else:
             raise CodepsHipError(f"{what}: gate is [{c}], one row per item of x's first dimension, or x's shape: got {tuple(gate.shape)} for {tuple(x.shape)}")
-    return _ChannelNorm.apply(x, residual, gate, weight, bias, next_weight, next_bias,
-                              (1, _NORM_KINDS[kind], eps, mode, _GATE_ACTS[gate_act], per_item, float(scale), _NORM_KINDS[next_kind], next_eps))
+    return _channel_norm_apply(x, residual, gate, weight, bias, next_weight, next_bias,
+                               (1, _NORM_KINDS[kind], eps, mode, _GATE_ACTS[gate_act], per_item, float(scale), _NORM_KINDS[next_kind], next_eps))
 
 
 # ---------------------------------------------------------------------------------------- optimiser
@@ -2571,27 +2593,32 @@ def _dense(t):
     return True
 
 
+def _types_of(tensors, device):
+    """Element types of a list of tensors as the C ABI's bytes; raises unless all are fp32, bf16 or fp16 on `device`."""
+    dtypes = {t.dtype for t in tensors}
+    if not dtypes <= _TYPES.keys() or set(map(torch.Tensor.get_device, tensors)) - {device.index}:
+        raise CodepsHipError(f"gradients are fp32, bf16 or fp16 tensors on {device}: got {sorted({(str(t.dtype), str(t.device)) for t in tensors})}")
+    return bytes([_TYPES[dtypes.pop()]]) * len(tensors) if len(dtypes) == 1 else bytes([_TYPES[t.dtype] for t in tensors])
+
+
 def grad_norm(grads, scale=1.0):
     """|scale g|_2 over a list of gradients (None entries are skipped), fp32 on the device: what AdamW clips by (C ABI: codeps_grad_norm).  fp32, bf16 and
     fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow."""
     grads = [g for g in grads if g is not None]
-    if not grads:
+    n = len(grads)
+    if n == 0:
         raise CodepsHipError("grad_norm: no gradients")
     dev = grads[0].device
     require_cuda(grads[0])
-    for i, g in enumerate(grads):
-        if g.dtype not in _TYPES or g.device != dev:
-            raise CodepsHipError(f"grad_norm: fp32, bf16 or fp16 tensors on one device, got {g.dtype} on {g.device}")
-        if not g.is_contiguous() and not _dense(g):
-            grads[i] = g.contiguous()
-    n = len(grads)
+    types = _types_of(grads, dev)
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    ptrs, numels = array.array("Q", map(torch.Tensor.data_ptr, grads)), array.array("q", map(torch.Tensor.numel, grads))
     out = torch.empty((), dtype=torch.float32, device=dev)
-    with _OnDevice(dev):
-        nbytes = lib().codeps_grad_norm_workspace_bytes(n)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib().codeps_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]), (ctypes.c_ubyte * n)(*[_TYPES[g.dtype] for g in grads]),
-                                     (ctypes.c_longlong * n)(*[g.numel() for g in grads]), n, float(scale), ptr(out), ptr(ws), nbytes, stream_ptr()),
-              "codeps_grad_norm")
+    nbytes = lib().codeps_grad_norm_workspace_bytes(n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "codeps_grad_norm", lib().codeps_grad_norm, ptrs.buffer_info()[0], types, numels.buffer_info()[0], n, float(scale), out.data_ptr(),
+            ws.data_ptr(), nbytes)
     return out
 
 

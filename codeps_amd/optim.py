@@ -7,12 +7,13 @@ Next to functional.adam_ema_step (Adam on flat fp32 buffers): decoupled weight d
 types, global-norm clipping inside the step, 8-bit states.  A step is two launches for all tensors (four with clipping), whatever their number up to 320.
 Step counts, the clipping factor and the random bits of the 8-bit rounding live on the device: a captured step() replays as the next step.
 """
+import array
 import ctypes
 
 import torch
 
 from . import functional as F
-from ._lib import AdamWGroup, CodepsHipError, check, lib, ptr, require_cuda, stream_ptr
+from ._lib import AdamWGroup, CodepsHipError, lib, ptr, require_cuda
 
 BLOCK = 256                     # elements of one tensor that share an exponent byte
 CHUNK = 2048                    # elements of one tensor that a work group updates
@@ -107,13 +108,11 @@ class AdamW:
         counts = torch.tensor([b - a for a, b in zip(chunk0, chunk0[1:])])
         self._chunk_items = torch.repeat_interleave(torch.arange(n, dtype=torch.int32), counts).to(dev) if chunk0[-1] else torch.zeros(1, dtype=torch.int32, device=dev)
         self._c_numels = (ctypes.c_longlong * n)(*self._numels)
-        self._c_grads, self._c_types = (ctypes.c_void_p * n)(), (ctypes.c_ubyte * n)()
         self._c_groups = (AdamWGroup * len(self.param_groups))()
         self._shapes = [p.shape for p in self.params]
         self._items = torch.zeros(n * lib().codeps_adamw_item_bytes(), dtype=torch.uint8, device=dev)
         self._fill_items()
-        with F._OnDevice(dev):
-            self._ws = torch.empty(lib().codeps_adamw_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        self._ws = torch.empty(lib().codeps_adamw_workspace_bytes(n), dtype=torch.uint8, device=dev)
 
     def _beside(self, tensors, dtypes, what):
         """ema / copies: one tensor (or None) per parameter, with its shape and layout."""
@@ -126,7 +125,7 @@ class AdamW:
         return tensors
 
     def _addresses(self):
-        return [t.data_ptr() for t in self.params]
+        return list(map(torch.Tensor.data_ptr, self.params))
 
     def _fill_items(self):
         """(Re)writes the device table in place: a captured step reads the same table."""
@@ -140,6 +139,9 @@ class AdamW:
                 raise CodepsHipError("codeps_adamw_item_fill: " + lib().codeps_last_error().decode())
         self._items.copy_(torch.frombuffer(bytearray(host.raw), dtype=torch.uint8))
         self._table_addresses = self._addresses()
+
+    def _states(self):
+        return self.exp_avg, self.exp_avg_sq, self.exp_avg_codes, self.exp_avg_exponents, self.root_codes, self.root_exponents
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -158,24 +160,28 @@ class AdamW:
         if len(grads) != len(params):
             raise CodepsHipError(f"AdamW.step: one gradient (or None) per parameter ({len(params)}), got {len(grads)}")
         some = [g for g in grads if g is not None]
-        if len(some) == len(params):
-            shapes = self._shapes
-        else:
-            shapes = [s for s, g in zip(self._shapes, grads) if g is not None]
-        if [g.shape for g in some] != shapes or {g.device for g in some} - {self.device} or {g.dtype for g in some} - set(F._TYPES):
-            raise CodepsHipError("AdamW.step: gradients have their parameter's shape and device, and are fp32, bf16 or fp16")
-        if not (all([g.is_contiguous() for g in some]) and all([p.is_contiguous() for p in params])):
+        whole = len(some) == len(params)
+        shapes = self._shapes if whole else [s for s, g in zip(self._shapes, grads) if g is not None]
+        if [g.shape for g in some] != shapes:
+            raise CodepsHipError("AdamW.step: gradients have their parameter's shape")
+        types = F._types_of(some, self.device)
+        if not (all(map(torch.Tensor.is_contiguous, some)) and all(map(torch.Tensor.is_contiguous, params))):
             if any(p.numel() != k or not F._dense(p) for p, k in zip(params, self._numels)):
                 raise CodepsHipError("AdamW.step: a parameter has changed its shape or layout since it was listed")
             grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
+            some = [g for g in grads if g is not None]
         if self._addresses() != self._table_addresses:
             if [p.shape for p in params] != self._shapes or any(p.dtype != torch.float32 or p.device != self.device for p in params):
                 raise CodepsHipError("AdamW.step: a parameter has changed its shape, type or device since it was listed")
             if torch.cuda.is_current_stream_capturing():
                 raise CodepsHipError("AdamW.step: a parameter has moved since the last step: run one step before the capture")
             self._fill_items()
-        self._c_grads[:] = [None if g is None else g.data_ptr() or 16 for g in grads]         # (an empty tensor has no address, but a gradient)
-        self._c_types[:] = [0 if g is None else F._TYPES[g.dtype] for g in grads]
+        # addresses and types of the gradients: 0 = none (an empty tensor has no address, but a gradient)
+        ptrs = array.array("Q", map(torch.Tensor.data_ptr, some) if whole else [0 if g is None else g.data_ptr() for g in grads])
+        if 0 in self._numels:
+            ptrs = array.array("Q", [0 if g is None else p or 16 for p, g in zip(ptrs, grads)])
+        if not whole:
+            types = bytes([0 if g is None else F._TYPES[g.dtype] for g in grads])
         for c, g in zip(self._c_groups, self.param_groups):
             lr = g["lr"]
             if torch.is_tensor(lr):
@@ -185,12 +191,10 @@ class AdamW:
             else:
                 c.lr, c.lr_device = lr, None
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
-        with F._OnDevice(self.device):
-            check(lib().codeps_adamw_step(ptr(self._items), len(params), ptr(self._chunk_items), self._chunk0, self._c_grads, self._c_types, self._c_numels,
-                                          self._c_groups, len(self.param_groups), ptr(self.steps), ptr(self.exp_avg), ptr(self.exp_avg_sq),
-                                          ptr(self.exp_avg_codes), ptr(self.exp_avg_exponents), ptr(self.root_codes), ptr(self.root_exponents),
-                                          float(grad_scale), self.max_norm or 0.0, int(self.skip_nonfinite), ptr(self.grad_norm), self.seed,
-                                          self.ema_alpha if apply_ema else -1.0, ptr(self._ws), self._ws.numel(), stream_ptr()), "codeps_adamw_step")
+        F._launch(self.device, "codeps_adamw_step", lib().codeps_adamw_step, self._items.data_ptr(), len(params), self._chunk_items.data_ptr(), self._chunk0,
+                  ptrs.buffer_info()[0], types, self._c_numels, self._c_groups, len(self.param_groups), self.steps.data_ptr(), *map(F._at, self._states()),
+                  float(grad_scale), self.max_norm or 0.0, int(self.skip_nonfinite), F._at(self.grad_norm), self.seed, self.ema_alpha if apply_ema else -1.0,
+                  self._ws.data_ptr(), self._ws.numel())
         torch.autograd.graph.increment_version(params)
         F.invalidate_weight_cache()
 
@@ -200,10 +204,8 @@ class AdamW:
             raise CodepsHipError("AdamW.moments_8bit: no tensor has 8-bit states")
         m = torch.empty(self._n8, dtype=torch.bfloat16, device=self.device)
         r = torch.empty_like(m)
-        with F._OnDevice(self.device):
-            check(lib().codeps_adamw_moments_8bit(ptr(self._items), len(self.params), ptr(self._chunk_items), self._n_chunks, ptr(self.exp_avg_codes),
-                                                  ptr(self.exp_avg_exponents), ptr(self.root_codes), ptr(self.root_exponents), ptr(m), ptr(r), stream_ptr()),
-                  "codeps_adamw_moments_8bit")
+        F._launch(self.device, "codeps_adamw_moments_8bit", lib().codeps_adamw_moments_8bit, self._items.data_ptr(), len(self.params),
+                  self._chunk_items.data_ptr(), self._n_chunks, *map(F._at, self._states()[2:]), m.data_ptr(), r.data_ptr())
         return m, r
 
     _STATES = ("steps", "exp_avg", "exp_avg_sq", "exp_avg_codes", "exp_avg_exponents", "root_codes", "root_exponents")
