@@ -2392,7 +2392,7 @@ def _pitched(t):
             span *= size
         if pitch is None:
             return t, c
-        if pitch >= c:
+        if c <= pitch < 1 << 24:
             return t, pitch
     return t.contiguous(), c
 
@@ -2562,6 +2562,8 @@ def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="lay
             mode = 1
         elif gate.shape == x.shape:
             mode = 3
+            if gate.dtype != x.dtype:
+                raise CodepsHipError(f"{what}: a gate of x's shape has x's type, got {gate.dtype} for {x.dtype}")
         elif (gate.dim() == 2 or gate.dim() == x.dim()) and gate.shape[0] == x.shape[0] and gate.numel() == gate.shape[0] * c and x.dim() > 2:
             mode, per_item = 2, max(1, x.numel() // c // max(1, x.shape[0]))
         else:

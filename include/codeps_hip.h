@@ -491,7 +491,7 @@ int codeps_adam_ema_step(float* params, const float* grads, float* exp_avg, floa
  *   n(v) = (v - mean v) / sqrt(var v + eps)  (LAYER)   |   v / sqrt(mean v^2 + eps)  (RMS)
  * x, h and dh have x_type; residual, y and dy res_type (x_type or F32); weight / bias, next_weight / next_bias and gate types of their own.  Every
  * vector is optional (NULL: weight 1, bias 0, residual 0).  gate: CHANNEL [channels], ITEM [rows / rows_per_item] rows, ELEMENT [rows] rows.
- * Pitches are elements from row to row (>= channels; rows may start at any element); outputs are dense.  Arithmetic fp32, one rounding per output.
+ * (an ELEMENT gate has x_type).  Pitches are elements from row to row (>= channels, below 2^24; rows may start at any element); outputs are dense.  Arithmetic fp32, one rounding per output.
  * stats (NULL in inference): [rows][4] floats (full = 0: [rows][2]), 16-byte aligned, handed unchanged to _bwd.
  * _bwd: dy / dh NULL = no gradient of that output (full = 1 needs one of them; with next_kind, dh).  Every gradient pointer may be NULL.  Gradients of
  * vectors are sums over rows in a fixed order, in the vector's type; the CODEPS_ACC_* bits add them to fp32 contents instead of storing them.

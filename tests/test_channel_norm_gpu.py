@@ -354,6 +354,17 @@ def test_gradients_go_straight_into_registered_sinks():
         assert torch.equal(flat[50 * i:50 * i + 50], torch.arange(50 * i, 50 * i + 50, dtype=F32, device=DEV) + want["d" + k]), k
 
 
+def test_rows_far_apart():
+    """Rows further apart than 32-bit offsets allow are copied, not misread."""
+    store = torch.zeros(2 * (1 << 24) + 40, dtype=BF16, device=DEV)
+    x = store.as_strided((3, 40), ((1 << 24), 1))
+    x.copy_(torch.randn(3, 40, device=DEV))
+    near = store.as_strided((2, 40), ((1 << 24) - 1, 1), 1)
+    near.copy_(torch.randn(2, 40, device=DEV))
+    for v in (x, near):
+        assert torch.equal(F.channel_norm(v), F.channel_norm(v.contiguous()))
+
+
 def test_rows_beyond_32_bit_offsets():
     """2^31 + elements: the last rows of a large map come out as they do alone."""
     C, rows = 2048, (1 << 20) + 3
@@ -376,7 +387,8 @@ def test_refusals():
                 lambda: F.channel_norm_residual(x, x.cpu()), lambda: F.channel_norm_residual(x, gate_act="silu"), lambda: F.channel_norm_residual(x, gate=w, gate_act="gelu"),
                 lambda: F.channel_norm_residual(x, gate=w[:4]), lambda: F.channel_norm_residual(x, gate=torch.zeros(2, 8, device=DEV)),
                 lambda: F.channel_norm_residual(x.view(2, 2, 8), gate=torch.zeros(2, 2, 2, 8, device=DEV)), lambda: F.channel_norm_residual(x, next_weight=w),
-                lambda: F.channel_norm_residual(x, next_kind="x"), lambda: F.channel_norm_residual(x, gate=w.double())):
+                lambda: F.channel_norm_residual(x, next_kind="x"), lambda: F.channel_norm_residual(x, gate=w.double()),
+                lambda: F.channel_norm_residual(x.half(), gate=x.float())):
         with pytest.raises(CodepsHipError):
             bad()
     leaf = x.clone().requires_grad_(True)

@@ -29,7 +29,7 @@ def _desc(**over):
 @pytest.mark.parametrize("over", [dict(rows=-1), dict(rows=1 << 31), dict(channels=0), dict(channels=8193), dict(x_type=3), dict(res_type=1), dict(x_type=1, res_type=2),
                                   dict(kind=3), dict(next_kind=-1), dict(gate_mode=4), dict(gate_act=3), dict(gate_mode=2, rows_per_item=0),
                                   dict(gate_mode=2, rows_per_item=3), dict(x_pitch=7), dict(res_pitch=7), dict(gate_mode=3, gate_pitch=7), dict(full=0, kind=0),
-                                  dict(full=0, next_kind=1), dict(full=0, gate_mode=1), dict(weight_type=9), dict(gate_type=-1)])
+                                  dict(full=0, next_kind=1), dict(gate_mode=3, gate_type=1), dict(x_pitch=1 << 24), dict(dy_pitch=1 << 24), dict(full=0, gate_mode=1), dict(weight_type=9), dict(gate_type=-1)])
 def test_channel_norm_descriptor_is_checked(over):
     lib, d, none = _lib.lib(), _desc(**over), [None] * 12
     assert lib.codeps_channel_norm_fwd(ctypes.byref(d), *none[:11]) == -1 and lib.codeps_last_error()
@@ -43,6 +43,7 @@ def test_channel_norm_null_pointers_and_workspaces_are_refused():
     assert lib.codeps_channel_norm_fwd(None, *[None] * 11) == -1
     assert lib.codeps_channel_norm_fwd(ctypes.byref(d), *[None] * 11) == -1
     assert lib.codeps_channel_norm_fwd(ctypes.byref(_desc(next_kind=1)), fake, fake, None, None, None, None, None, fake, None, None, None) == -1
+    assert lib.codeps_channel_norm_fwd(ctypes.byref(_desc(x_type=1)), fake, None, None, None, None, None, None, fake, None, None, None) == -1     # y in fp32 without a residual
     assert lib.codeps_channel_norm_fwd(ctypes.byref(_desc(gate_mode=1)), fake, fake, None, None, None, None, None, fake, None, None, None) == -1
     need = lib.codeps_channel_norm_bwd_workspace_bytes(ctypes.byref(d))
     assert need > 0
