@@ -15,6 +15,7 @@
 // result can differ from the exact one only where the sum lies within two units of a multiple of 65536: there (about 8 elements in 100 000) the
 // moments are formed again in 64 bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -22,6 +23,7 @@ namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int CHUNK = 2048, QB = 256, THREADS = 256, PER_LAUNCH = 320;
 constexpr int MANT_M = 3, MANT_R = 4;
@@ -64,30 +66,10 @@ __device__ __forceinline__ float grad_at(const void* g, int type, long long i) {
     const unsigned short h = ((const unsigned short*)g)[i];
     return type == CODEPS_BF16 ? __uint_as_float((unsigned)h << 16) : (float)__builtin_bit_cast(_Float16, h);
 }
-// four gradients from i on; the ones from n on are zero
-__device__ __forceinline__ void grad4(const void* g, int type, long long i, long long n, float* o) {
-    if (i + 4 <= n) {
-        if (type == CODEPS_F32) {
-            const f32x4u q = *reinterpret_cast<const f32x4u*>((const float*)g + i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = q[e];
-        } else {
-            const u16x4u q = *reinterpret_cast<const u16x4u*>((const unsigned short*)g + i);
-            if (type == CODEPS_BF16) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = __uint_as_float((unsigned)q[e] << 16);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)q[e]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = i + e < n ? grad_at(g, type, i + e) : 0.f;
-    }
-}
-__device__ __forceinline__ void load4(const float* p, long long i, long long n, float* o) {
-    if (i + 4 <= n) {
+// Four elements from i on.  TAIL: the ones from n on read as zero and are not stored; otherwise all four are inside (no branch: a branch per load makes the
+// compiler wait for each one before the next).
+template <bool TAIL> __device__ __forceinline__ void load4(const float* p, long long i, long long n, float* o) {
+    if (!TAIL || i + 4 <= n) {
         const f32x4u q = *reinterpret_cast<const f32x4u*>(p + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = q[e];
@@ -96,8 +78,8 @@ __device__ __forceinline__ void load4(const float* p, long long i, long long n, 
         for (int e = 0; e < 4; ++e) o[e] = i + e < n ? p[i + e] : 0.f;
     }
 }
-__device__ __forceinline__ void store4(float* p, long long i, long long n, const float* v) {
-    if (i + 4 <= n) {
+template <bool TAIL> __device__ __forceinline__ void store4(float* p, long long i, long long n, const float* v) {
+    if (!TAIL || i + 4 <= n) {
         f32x4u q;
 #pragma unroll
         for (int e = 0; e < 4; ++e) q[e] = v[e];
@@ -108,12 +90,29 @@ __device__ __forceinline__ void store4(float* p, long long i, long long n, const
             if (i + e < n) p[i + e] = v[e];
     }
 }
+template <bool TAIL> __device__ __forceinline__ void grad4(const void* g, int type, long long i, long long n, float* o) {
+    if (type == CODEPS_F32) {
+        load4<TAIL>((const float*)g, i, n, o);
+    } else if (!TAIL || i + 4 <= n) {
+        const u16x4u q = *reinterpret_cast<const u16x4u*>((const unsigned short*)g + i);
+        if (type == CODEPS_BF16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __uint_as_float((unsigned)q[e] << 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)q[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = i + e < n ? grad_at(g, type, i + e) : 0.f;
+    }
+}
 __device__ __forceinline__ unsigned short narrow16(float v, int type) {
     return type == CODEPS_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v) : __builtin_bit_cast(unsigned short, (_Float16)v);
 }
-__device__ __forceinline__ void store4_16(void* p, int type, long long i, long long n, const float* v) {
+template <bool TAIL> __device__ __forceinline__ void store4_16(void* p, int type, long long i, long long n, const float* v) {
     unsigned short* d = (unsigned short*)p + i;
-    if (i + 4 <= n) {
+    if (!TAIL || i + 4 <= n) {
         u16x4u q;
 #pragma unroll
         for (int e = 0; e < 4; ++e) q[e] = narrow16(v[e], type);
@@ -152,13 +151,17 @@ __global__ __launch_bounds__(THREADS) void grad_norm_kernel(NormTensors t, doubl
         const void* g = t.g[lo];
         const long long n = t.n[lo], i0 = (long long)(c - t.chunk0[lo]) * NCHUNK + threadIdx.x * 4;
         const int type = t.type[lo];
-        float v[NCHUNK / (THREADS * 4)][4];
+        const auto chunk = [&](auto tail) {
+            float v[NCHUNK / (THREADS * 4)][4];
 #pragma unroll
-        for (int k = 0; k < NCHUNK / (THREADS * 4); ++k) grad4(g, type, i0 + k * THREADS * 4, n, v[k]);
+            for (int k = 0; k < NCHUNK / (THREADS * 4); ++k) grad4<decltype(tail)::value>(g, type, i0 + k * THREADS * 4, n, v[k]);
 #pragma unroll
-        for (int k = 0; k < NCHUNK / (THREADS * 4); ++k)
+            for (int k = 0; k < NCHUNK / (THREADS * 4); ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += (double)v[k][e] * (double)v[k][e];
+                for (int e = 0; e < 4; ++e) s[e] += (double)v[k][e] * (double)v[k][e];
+        };
+        if ((long long)(c - t.chunk0[lo] + 1) * NCHUNK <= n) chunk(std::false_type{});
+        else chunk(std::true_type{});
     }
     const double sum = block_sum64((s[0] + s[1]) + (s[2] + s[3]), red);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -220,24 +223,21 @@ template <int MANT> __device__ __forceinline__ int unit_of(unsigned top) {
 }
 // a code's bits, shifted to where fp32 has exponent and mantissa, are the value times 2^-112 -- field 0 included, as fp32's own subnormals
 template <int MANT> __device__ __forceinline__ float decode(unsigned code, int unit) {
-    return unit == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(__uint_as_float(code << (23 - MANT)), unit - 15);
+    return __builtin_ldexpf(__uint_as_float(code << (23 - MANT)), unit - 15);            // (a block that is not finite holds zeros: its caller makes them NaN)
 }
-template <int MANT, typename T> __device__ __forceinline__ int step_exponent(T a, int unit) {          // log2 of the quantum around a, in block units
-    const int e = a == (T)0 ? -14 : (sizeof(T) == 4 ? __builtin_amdgcn_frexp_expf((float)a) : __builtin_amdgcn_frexp_exp((double)a)) - 1 + 127 - unit;
-    return max(e, -14);
-}
-// |x| = a -> code.  slack: how far (in 2^-16 quanta) a may be from the exact value; unsure: whether that could change the code.
-template <int MANT> __device__ __forceinline__ unsigned encode(float a, int unit, unsigned rho, unsigned slack, bool& unsure) {
-    a = unit == 0 ? 0.f : a;
-    const int low = step_exponent<MANT, float>(a, unit);
-    const unsigned k = (unsigned)ldexpf(a, 127 - unit + MANT - low + 16) + rho;
+// log2 of the quantum at |x| = a, in units of the block (fp32: a's biased exponent is good enough, units from 14 on have nothing smaller than a subnormal code
+// that they could not hold)
+template <int MANT> __device__ __forceinline__ int place_of(float a, int unit) { return max((int)(__float_as_uint(a) >> 23) - unit, -14); }
+// |x| = a -> code at place `low`.  slack: how far (in 2^-16 quanta) a may be from the exact value; unsure: whether that could change the code.
+template <int MANT> __device__ __forceinline__ unsigned encode(float a, int unit, int low, unsigned rho, unsigned slack, bool& unsure) {
+    const unsigned k = (unsigned)__builtin_ldexpf(a, 143 + MANT - unit - low) + rho;
     unsure = ((k + slack) & 0xffffu) <= 2 * slack;
     return ((unsigned)(low + 14) << MANT) + (k >> 16);
 }
 template <int MANT> __device__ __forceinline__ unsigned encode64(double a, int unit, unsigned rho) {
     a = unit == 0 ? 0.0 : a;
-    const int low = step_exponent<MANT, double>(a, unit);
-    const unsigned k = (unsigned)ldexp(a, 127 - unit + MANT - low + 16) + rho;
+    const int low = a == 0.0 ? -14 : max(__builtin_amdgcn_frexp_exp(a) - 1 + 127 - unit, -14);
+    const unsigned k = (unsigned)ldexp(a, 143 + MANT - unit - low) + rho;
     return min(((unsigned)(low + 14) << MANT) + (k >> 16), (16u << MANT) - 1u);
 }
 __device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsigned k1) {
@@ -247,14 +247,127 @@ __device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsign
     x *= 0x846CA68Bu;
     return x ^ (x >> 16);
 }
+// largest of a wave's values, in every lane: lanes 1, 2, 4, 8 away over DPP, 16 and 32 away by exchanging half rows
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
-    return v;
+    v = dpp_max<0xB1>(v);
+    v = dpp_max<0x4E>(v);
+    v = dpp_max<0x141>(v);
+    v = dpp_max<0x140>(v);
+    u32x2 q = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(q[0], q[1]);
+    q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)max(q[0], q[1]));
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ the update
 struct States { float *m, *v; unsigned char *mc, *me, *rc, *re; };
+
+// one chunk of a tensor; WIDE: 32-bit states.  The gradients are loaded last: their type is known at run time, and where the branches meet the compiler waits.
+template <bool WIDE, bool TAIL>
+__device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, const void* gp, int gt, float* const ema, long long start, const States& st, float al, float oal) {
+    constexpr int K = CHUNK / (THREADS * 4);
+    const long long n = it.n, first = start + (long long)threadIdx.x * 4;
+    float p[K][4], g[K][4], a[K][4], b[K][4], em[K][4];
+    unsigned mc[K], rc[K];
+    int mu[K], ru[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = first + k * THREADS * 4;
+        load4<TAIL>(it.p, i, n, p[k]);
+        if (ema) load4<TAIL>(ema, i, n, em[k]);
+        if constexpr (WIDE) {
+            load4<TAIL>(st.m + it.off, i, n, a[k]);
+            load4<TAIL>(st.v + it.off, i, n, b[k]);
+        } else if (!TAIL || (i & ~(long long)(QB - 1)) < n) {                  // the same for a whole wave: it owns the 256 elements from here on
+            const long long q = it.off + i;
+            mc[k] = *reinterpret_cast<const unsigned*>(st.mc + q);
+            rc[k] = *reinterpret_cast<const unsigned*>(st.rc + q);
+            const long long blk = (it.off + start + k * THREADS * 4) / QB + (threadIdx.x >> 6);
+            mu[k] = st.me[blk];
+            ru[k] = st.re[blk];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) grad4<TAIL>(gp, gt, first + k * THREADS * 4, n, g[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const long long i = first + k * THREADS * 4;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float gg = g[k][e] * f.fgs;
+                a[k][e] = f.fb1 * a[k][e] + f.fob1 * gg;
+                b[k][e] = f.fb2 * b[k][e] + f.fob2 * gg * gg;
+                p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(sqrtf(b[k][e]) * f.root + f.eps);
+            }
+            store4<TAIL>(st.m + it.off, i, n, a[k]);
+            store4<TAIL>(st.v + it.off, i, n, b[k]);
+        } else {
+            if (TAIL && (i & ~(long long)(QB - 1)) >= n) continue;
+            const int um = __builtin_amdgcn_readfirstlane(mu[k]), ur = __builtin_amdgcn_readfirstlane(ru[k]);
+            const float bad_m = um == 255 ? __uint_as_float(0x7fc00000u) : 0.f, bad_r = ur == 255 ? __uint_as_float(0x7fc00000u) : 0.f;
+            float m0[4], r0[4], c[4];
+            unsigned mtop = 0, rtop = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned code = mc[k] >> (8 * e);
+                const float q = decode<MANT_M>(code & 127u, um) + bad_m;
+                m0[e] = __uint_as_float(__float_as_uint(q) | (code & 128u) << 24);
+                r0[e] = decode<MANT_R>(rc[k] >> (8 * e) & 255u, ur) + bad_r;
+                const float gg = g[k][e] * f.fgs;
+                c[e] = f.fob1 * gg;
+                a[k][e] = __builtin_fmaf(f.fb1, m0[e], c[e]);
+                b[k][e] = __builtin_amdgcn_sqrtf(__builtin_fmaf(f.fb2, r0[e] * r0[e], f.fob2 * gg * gg));
+                p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(b[k][e] * f.root + f.eps);
+                mtop = max(mtop, __float_as_uint(a[k][e]) & 0x7fffffffu);
+                rtop = max(rtop, __float_as_uint(b[k][e]) & 0x7fffffffu);
+            }
+            const int nm = unit_of<MANT_M>(wave_umax(mtop)), nr = unit_of<MANT_R>(wave_umax(rtop));
+            const bool small = nm < 14 || nr < 14;                             // (a block of nearly nothing: all of it in 64 bits)
+            unsigned ncm = 0, ncr = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned rnd = random_bits(i + e, f.k0, f.k1);
+                bool dm, dr;
+                // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
+                const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(c[e]);
+                const int low = place_of<MANT_M>(am, nm);
+                const unsigned slack = 2u + (unsigned)fminf(__builtin_ldexpf(size, 143 + MANT_M - 22 - nm - low), 32000.f);
+                bool minus = a[k][e] < 0.f;
+                unsigned cm = encode<MANT_M>(am, nm, low, rnd & 0xffffu, slack, dm);
+                unsigned cr = encode<MANT_R>(b[k][e], nr, place_of<MANT_R>(b[k][e], nr), rnd >> 16, 2u, dr);
+                if (dm || dr || small) {
+                    const double gg = (double)g[k][e] * f.gs;
+                    const double m = f.b1 * (double)m0[e] + f.ob1 * gg;
+                    minus = m < 0.0;
+                    cm = encode64<MANT_M>(fabs(m), nm, rnd & 0xffffu);
+                    cr = encode64<MANT_R>(sqrt(f.b2 * ((double)r0[e] * (double)r0[e]) + f.ob2 * gg * gg), nr, rnd >> 16);
+                }
+                ncm |= (cm | (minus ? 128u : 0u)) << (8 * e);
+                ncr |= cr << (8 * e);
+            }
+            if (nm == 255) ncm = 0;
+            if (nr == 255) ncr = 0;
+            const long long q = it.off + i;
+            *reinterpret_cast<unsigned*>(st.mc + q) = ncm;
+            *reinterpret_cast<unsigned*>(st.rc + q) = ncr;
+            if ((threadIdx.x & 63) == 0) {
+                st.me[q / QB] = (unsigned char)nm;
+                st.re[q / QB] = (unsigned char)nr;
+            }
+        }
+        store4<TAIL>(it.p, i, n, p[k]);
+        if (it.copy) store4_16<TAIL>(it.copy, it.copy_type, i, n, p[k]);
+        if (ema) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) em[k][e] = al * em[k][e] + oal * p[k][e];
+            store4<TAIL>(ema, i, n, em[k]);
+        }
+    }
+}
 
 __global__ __launch_bounds__(THREADS) void adamw_step_kernel(Grads grads, const Item* __restrict__ items, const int* __restrict__ chunk_items,
                                                              const Factors* __restrict__ factors, int base, long long first_chunk, States st, float al, float oal) {
@@ -264,100 +377,28 @@ __global__ __launch_bounds__(THREADS) void adamw_step_kernel(Grads grads, const 
     const Factors& f = factors[t];
     float* const ema = al >= 0.f ? it.ema : nullptr;
     if (f.skipped || (!f.live && !ema)) return;
-    const long long n = it.n, start = (chunk - it.chunk0) * CHUNK;
-    constexpr int K = CHUNK / (THREADS * 4);
-    float p[K][4], g[K][4], a[K][4], b[K][4], em[K][4];
+    const long long start = (chunk - it.chunk0) * CHUNK;
+    if (!f.live) {                                                             // no gradient: the average follows the parameter as it is
+        for (int k = 0; k < CHUNK / (THREADS * 4); ++k) {
+            const long long i = start + (k * THREADS + threadIdx.x) * 4;
+            float p[4], em[4];
+            load4<true>(it.p, i, it.n, p);
+            load4<true>(ema, i, it.n, em);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) em[e] = al * em[e] + oal * p[e];
+            store4<true>(ema, i, it.n, em);
+        }
+        return;
+    }
     const void* gp = grads.g[t - base];
     const int gt = grads.type[t - base];
-    const bool wide = it.bits == 32;
-    unsigned mc[K], rc[K];
-    int mu[K], ru[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const long long i = start + k * THREADS * 4 + threadIdx.x * 4;
-        load4(it.p, i, n, p[k]);
-        if (ema) load4(ema, i, n, em[k]);
-        if (!f.live) continue;
-        grad4(gp, gt, i, n, g[k]);
-        if (wide) {
-            load4(st.m + it.off, i, n, a[k]);
-            load4(st.v + it.off, i, n, b[k]);
-        } else if ((i & ~(long long)(QB - 1)) < n) {
-            const long long q = it.off + i;
-            mc[k] = *reinterpret_cast<const unsigned*>(st.mc + q);
-            rc[k] = *reinterpret_cast<const unsigned*>(st.rc + q);
-            mu[k] = st.me[q / QB];
-            ru[k] = st.re[q / QB];
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const long long i = start + k * THREADS * 4 + threadIdx.x * 4;
-        if (f.live) {
-            if (wide) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float gg = g[k][e] * f.fgs;
-                    a[k][e] = f.fb1 * a[k][e] + f.fob1 * gg;
-                    b[k][e] = f.fb2 * b[k][e] + f.fob2 * gg * gg;
-                    p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(sqrtf(b[k][e]) * f.root + f.eps);
-                }
-                store4(st.m + it.off, i, n, a[k]);
-                store4(st.v + it.off, i, n, b[k]);
-            } else if ((i & ~(long long)(QB - 1)) < n) {                        // the same for a whole wave: it owns this block
-                float m0[4], r0[4];
-                unsigned mtop = 0, rtop = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned c = mc[k] >> (8 * e) & 255u;
-                    const float q = decode<MANT_M>(c & 127u, mu[k]);
-                    m0[e] = c & 128u ? -q : q;
-                    r0[e] = decode<MANT_R>(rc[k] >> (8 * e) & 255u, ru[k]);
-                    const float gg = g[k][e] * f.fgs;
-                    a[k][e] = f.fb1 * m0[e] + f.fob1 * gg;
-                    const float v = f.fb2 * (r0[e] * r0[e]) + f.fob2 * gg * gg;
-                    b[k][e] = sqrtf(v);
-                    p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(b[k][e] * f.root + f.eps);
-                    mtop = max(mtop, __float_as_uint(a[k][e]) & 0x7fffffffu);
-                    rtop = max(rtop, __float_as_uint(b[k][e]) & 0x7fffffffu);
-                }
-                mu[k] = unit_of<MANT_M>(wave_umax(mtop));
-                ru[k] = unit_of<MANT_R>(wave_umax(rtop));
-                unsigned ncm = 0, ncr = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned rnd = random_bits(i + e, f.k0, f.k1);
-                    bool um, ur;
-                    // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
-                    const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(f.fob1 * g[k][e] * f.fgs);
-                    const int low = step_exponent<MANT_M, float>(mu[k] == 0 ? 0.f : am, mu[k]);
-                    const unsigned slack = 2u + (unsigned)fminf(ldexpf(size, 127 - mu[k] + MANT_M - low + 16 - 22), 32000.f);
-                    unsigned cm = encode<MANT_M>(am, mu[k], rnd & 0xffffu, slack, um);
-                    unsigned cr = encode<MANT_R>(b[k][e], ru[k], rnd >> 16, 2u, ur);
-                    if (um || ur) {
-                        const double gg = (double)g[k][e] * f.gs;
-                        if (um) cm = encode64<MANT_M>(fabs(f.b1 * (double)m0[e] + f.ob1 * gg), mu[k], rnd & 0xffffu);
-                        if (ur) cr = encode64<MANT_R>(sqrt(f.b2 * ((double)r0[e] * (double)r0[e]) + f.ob2 * gg * gg), ru[k], rnd >> 16);
-                    }
-                    ncm |= ((mu[k] == 255 ? 0u : cm & 127u) | (a[k][e] < 0.f ? 128u : 0u)) << (8 * e);
-                    ncr |= (ru[k] == 255 ? 0u : cr & 255u) << (8 * e);
-                }
-                const long long q = it.off + i;
-                *reinterpret_cast<unsigned*>(st.mc + q) = ncm;
-                *reinterpret_cast<unsigned*>(st.rc + q) = ncr;
-                if ((threadIdx.x & 63) == 0) {
-                    st.me[q / QB] = (unsigned char)mu[k];
-                    st.re[q / QB] = (unsigned char)ru[k];
-                }
-            }
-            store4(it.p, i, n, p[k]);
-            if (it.copy) store4_16(it.copy, it.copy_type, i, n, p[k]);
-        }
-        if (ema) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) em[k][e] = al * em[k][e] + oal * p[k][e];
-            store4(ema, i, n, em[k]);
-        }
+    const bool whole = start + CHUNK <= it.n;
+    if (it.bits == 32) {
+        if (whole) update_chunk<true, false>(it, f, gp, gt, ema, start, st, al, oal);
+        else update_chunk<true, true>(it, f, gp, gt, ema, start, st, al, oal);
+    } else {
+        if (whole) update_chunk<false, false>(it, f, gp, gt, ema, start, st, al, oal);
+        else update_chunk<false, true>(it, f, gp, gt, ema, start, st, al, oal);
     }
 }
 
@@ -374,16 +415,17 @@ __global__ __launch_bounds__(THREADS) void adamw_moments_kernel(const Item* __re
         if (i >= n) continue;
         const unsigned cm = *reinterpret_cast<const unsigned*>(mc + q), cr = *reinterpret_cast<const unsigned*>(rc + q);
         const int mu = me[q / QB], ru = re[q / QB];
+        const float bad_m = mu == 255 ? __uint_as_float(0x7fc00000u) : 0.f, bad_r = ru == 255 ? __uint_as_float(0x7fc00000u) : 0.f;
         float m[4], r[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const unsigned c = cm >> (8 * e) & 255u;
-            const float v = decode<MANT_M>(c & 127u, mu);
+            const float v = decode<MANT_M>(c & 127u, mu) + bad_m;
             m[e] = c & 128u ? -v : v;
-            r[e] = decode<MANT_R>(cr >> (8 * e) & 255u, ru);
+            r[e] = decode<MANT_R>(cr >> (8 * e) & 255u, ru) + bad_r;
         }
-        store4_16((unsigned short*)om + it.packed, CODEPS_BF16, i, n, m);
-        store4_16((unsigned short*)orr + it.packed, CODEPS_BF16, i, n, r);
+        store4_16<true>((unsigned short*)om + it.packed, CODEPS_BF16, i, n, m);
+        store4_16<true>((unsigned short*)orr + it.packed, CODEPS_BF16, i, n, r);
     }
 }
 
