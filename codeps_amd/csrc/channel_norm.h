@@ -253,7 +253,7 @@ inline Plan plan_of(const codeps_channel_norm_desc* d, int want, int resident) {
     const bool per_item = d->gate_mode == CODEPS_GATE_ITEM;
     p.rpi = per_item ? d->rows_per_item : (int)d->rows;
     p.items = per_item ? std::max(1, (int)(d->rows / d->rows_per_item)) : 1;
-    const int most = std::max(1, cdiv(p.rpi, p.s.rpb));
+    const int most = (int)std::max<long long>(1, ((long long)p.rpi + p.s.rpb - 1) / p.s.rpb);
     p.slices = std::max(1, std::min(most, want / p.items));
     p.blocks = std::min(p.items, std::max(1, resident / p.slices)) * p.slices;
     return p;

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
     }
     const int S = a.slices, slice = (int)(blockIdx.x % (unsigned)S);
     const bool has_r = a.r != nullptr;
-    for (int item = (int)(blockIdx.x / (unsigned)S); item < a.items; item += (int)(gridDim.x / (unsigned)S)) {
+    for (unsigned item = blockIdx.x / (unsigned)S; item < (unsigned)a.items; item += gridDim.x / (unsigned)S) {
         if constexpr (HELD) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256) void channel_norm_columns_kernel(Args a) {
     load_vector<V>(a.b, a.wt, 0, c0, C, 0.f, b);
     load_vector<V>(a.nw, a.nt, 0, c0, C, 1.f, nw);
     const bool has_r = a.r != nullptr;
-    for (int item = (int)(blockIdx.x / (unsigned)S); item < a.items; item += (int)(gridDim.x / (unsigned)S)) {
+    for (unsigned item = blockIdx.x / (unsigned)S; item < (unsigned)a.items; item += gridDim.x / (unsigned)S) {
         if constexpr (HELD) {
             load_vector<V>(a.gate, a.gt, (size_t)item * a.gp, c0, C, 0.f, gv);
 #pragma unroll
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void channel_norm_columns_kernel(Args a) {
                 ag[e] = 0.f;
             }
         }
-        for (int i = slice; i < a.rpi; i += S) {
+        for (long long i = slice; i < a.rpi; i += S) {
             const size_t row = (size_t)item * a.rpi + i;
             const TX* px = (const TX*)a.x + row * a.xp;
             float u[V], d[V];
@@ -434,15 +434,15 @@ extern "C" int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const 
     }
     if (columns && (d->rows > 0 || d->gate_mode == CODEPS_GATE_CHANNEL)) add(gate_slab, dgate, d->gate_type, p.items, p.slices, C, 0);
     // (items behind the 65535th have their own launch: a grid's second dimension ends there)
-    for (int g0 = 0; k > 0 && g0 < groups; g0 += 65535) {
+    for (long long g0 = 0; k > 0 && g0 < groups; g0 += 65535) {
         Finish part = f;
         for (int i = 0; i < k; ++i) {
-            const int skip = std::min(g0, f.groups[i]);
+            const int skip = (int)std::min<long long>(g0, f.groups[i]);
             part.groups[i] = std::min(f.groups[i] - skip, 65535);
             part.part[i] = f.part[i] + (size_t)skip * f.n[i] * f.pitch[i];
             part.out[i] = (char*)f.out[i] + (size_t)skip * C * (f.type[i] == CODEPS_F32 ? 4 : 2);
         }
-        hipLaunchKernelGGL(channel_norm_finish_kernel, dim3(cdiv(C, 16), std::min(groups - g0, 65535), k), dim3(16 * FINISH_STREAMS), 0, st, part);
+        hipLaunchKernelGGL(channel_norm_finish_kernel, dim3(cdiv(C, 16), (unsigned)std::min<long long>(groups - g0, 65535), k), dim3(16 * FINISH_STREAMS), 0, st, part);
         CODEPS_CHECK_LAUNCH("channel_norm_finish_kernel");
     }
     return CODEPS_OK;

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : WAVE_THREADS) void channel_norm_fwd_
     }
     const int S = a.slices, slice = (int)(blockIdx.x % (unsigned)S);
     const bool has_r = a.r != nullptr;
-    for (int item = (int)(blockIdx.x / (unsigned)S); item < a.items; item += (int)(gridDim.x / (unsigned)S)) {
+    for (unsigned item = blockIdx.x / (unsigned)S; item < (unsigned)a.items; item += gridDim.x / (unsigned)S) {
         if constexpr (FULL && GATE == GATE_HELD) {
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {

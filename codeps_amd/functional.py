@@ -2468,7 +2468,8 @@ def _channel_norm_bwd(ctx, *douts):
         d.next_kind = 0
         residual = None
     dx = x.new_empty(x.shape) if need[0] else None
-    dres = torch.empty(x.shape, dtype=ctx.res_dtype, device=dev) if need[1] else None
+    # without a next norm y's gradient is the residual's: handed on, not copied
+    dres = torch.empty(x.shape, dtype=ctx.res_dtype, device=dev) if need[1] and d.next_kind else None
     dgate = (gate.new_empty if d.rows else gate.new_zeros)(ctx.gate_shape) if need[2] else None
     outs, acc = [None] * 4, 0
     for i in range(4 if d.next_kind else 2):
@@ -2485,7 +2486,7 @@ def _channel_norm_bwd(ctx, *douts):
             _at(next_weight), stats.data_ptr(), _at(dy), _at(dh), _at(dx), _at(dres), _at(dgate), _at(outs[0]), _at(outs[1]), _at(outs[2]), _at(outs[3]),
             acc, ws.data_ptr(), nbytes)
     outs = [None if sinks[i] is not None else outs[i] for i in range(4)]
-    return (dx, dres, dgate, *outs, None)
+    return (dx, dres if d.next_kind or not need[1] else douts[0], dgate, *outs, None)
 
 
 _channel_norm_bwd_once = torch.autograd.function.once_differentiable(_channel_norm_bwd)

@@ -173,6 +173,19 @@ def test_steps_against_64_bits(bits, dtype):
         assert abs(float(opt.grad_norm) - plain.norm) <= 2 * U * plain.norm
 
 
+def test_eight_bits_for_the_smallest_tensors():
+    """Tensors shorter than a block, of one element, and empty ones, all in 8 bits."""
+    params = tensors([1, 5, (0,), 300, 255, 2], 8, 0.1)
+    opt = AdamW(params, lr=1e-2, state_bits=8, small_numel=0, max_norm=1e-3, seed=4)
+    plain = Plain(params, [0.01] * 6, [8] * 6, 1e-2, (0.9, 0.999), 1e-8, 1e-3, seed=4)
+    for k in range(3):
+        grads = gradients(params, 30 + k, F16)
+        opt.step(grads)
+        plain.step(grads)
+        check(opt, plain)
+    assert opt.exp_avg is None and opt.moments_8bit()[0].numel() == 563
+
+
 def test_default_gradients_mixed_types_and_zero_grad():
     params = [torch.nn.Parameter(p) for p in tensors([300, (7, 9), 4], 3)]
     opt = AdamW(params, lr=1e-2, weight_decay=0.0)
