@@ -21,6 +21,7 @@ namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));              // rows start at any multiple of the element size
 typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 struct bf16 { unsigned short v; };
@@ -81,14 +82,33 @@ template <int V, bool TAIL, typename T> __device__ __forceinline__ void load_pie
     if constexpr (!TAIL) {
         load_full<V>(at(row, off + (c0 < C ? c0 : 0)), o);
     } else if (C >= V) {
+        // the shift works on the loaded words, two 16-bit elements at a time
+        constexpr int PER = sizeof(T) == 4 ? 1 : 2, W = V / PER;              // elements per word, words
         const int first = min(c0, C - V), sh = c0 - first;
-        load_full<V>(at(row, off + first), o);
+        const T* p = at(row, off + first);
+        unsigned r[W];
 #pragma unroll
-        for (int s = 1; s < V; s *= 2)
+        for (int k = 0; k < W / 4; ++k) {
+            const u32x4u q = *reinterpret_cast<const u32x4u*>(reinterpret_cast<const char*>(p) + 16 * k);
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = (sh & s) ? (e + s < V ? o[e + s] : 0.f) : o[e];
+            for (int e = 0; e < 4; ++e) r[4 * k + e] = q[e];
+        }
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = sh >= V ? 0.f : o[e];
+        for (int s = W / 2; s > 0; s /= 2)
+#pragma unroll
+            for (int e = 0; e < W; ++e) r[e] = (sh & (s * PER)) ? (e + s < W ? r[e + s] : 0u) : r[e];
+        if constexpr (PER == 2) {
+            const unsigned bits = (sh & 1) * 16;
+#pragma unroll
+            for (int e = 0; e < W; ++e) r[e] = __builtin_amdgcn_alignbit(e + 1 < W ? r[e + 1] : 0u, r[e], bits);
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) r[e] = sh >= V ? 0u : r[e];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if constexpr (PER == 1) o[e] = __uint_as_float(r[e]);
+            else o[e] = widen(T{(unsigned short)(e % 2 ? r[e / 2] >> 16 : r[e / 2] & 0xffffu)});
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = c0 + e < C ? widen(at(row, off + c0)[e]) : 0.f;
@@ -97,10 +117,21 @@ template <int V, bool TAIL, typename T> __device__ __forceinline__ void load_pie
 template <int V, bool TAIL, typename T> __device__ __forceinline__ void store_piece(T* row, int off, int c0, int C, const float* v) {
     if (c0 + V <= C) {
         store_full<V>(at(row, off + c0), v);
-    } else if constexpr (TAIL) {
+    } else if constexpr (TAIL) {                                     // V / 2, V / 4, .. elements at a time, by the bits of what is left
+        const int left = max(C - c0, 0);
+        T* p = at(row, off + c0);
+        T t[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (c0 + e < C) narrow(v[e], at(row, off + c0)[e]);
+        for (int e = 0; e < V; ++e) narrow(v[e], t[e]);
+#pragma unroll
+        for (int n = V / 2; n > 0; n /= 2) {
+            if (left & n) {
+                __builtin_memcpy(p, t, n * sizeof(T));
+                p += n;
+#pragma unroll
+                for (int e = 0; e < n; ++e) t[e] = t[e + n];
+            }
+        }
     }
 }
 // a vector [C] of a type known at run time (outside the row loop); absent: fill
@@ -129,7 +160,7 @@ struct Args {
     float *stats, *slab, *gate_slab, *row_sums;
     const float* stats_in;
     long long rows, xp, rp, gp, dyp, dhp;
-    int C, kind, next, act, rpi, wt, gt, nt, lpr_log2, items, slices, cols;      // cols: which column sums are wanted (COL_*)
+    int C, kind, next, act, rpi, shared_lines, wt, gt, nt, lpr_log2, items, slices, cols;      // cols: which column sums are wanted (COL_*)
     float scale, eps, neps, inv_c;
 };
 enum { COL_W = 1, COL_B = 2, COL_NW = 4, COL_NB = 8, COL_G = 16 };
@@ -143,6 +174,14 @@ template <bool BLOCK> __device__ __forceinline__ Place place_of(int lpr_log2) {
     if constexpr (BLOCK) return {(int)blockDim.x, (int)threadIdx.x, 0, 0, 1};
     const int per_wave = 64 >> lpr_log2, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), in_wave = (int)threadIdx.x & 63;
     return {1 << lpr_log2, in_wave & ((1 << lpr_log2) - 1), wave * per_wave, in_wave >> lpr_log2, WAVE_THREADS >> lpr_log2};
+}
+
+// The slice of a block.  Blocks go to the 8 XCDs in turn.  Where a row is not a whole number of 128-byte lines, neighbouring slices, whose rows share lines, are
+// given to blocks of one XCD, and its L2 merges their parts of a line: 32768 x 1000 bf16, forward and backward 87 -> 82 us; whole lines are better off in
+// turn (262144 x 256 bf16 131 against 137 us).
+__device__ __forceinline__ int slice_of(unsigned block, int S, bool shared_lines) {
+    const int s = (int)(block % (unsigned)S);
+    return shared_lines && S % 8 == 0 ? (s & 7) * (S >> 3) + (s >> 3) : s;
 }
 
 // ---- sums over the lanes that share a row: lanes 1, 2, 4, 8 away over DPP, 16 and 32 away by exchanging half rows (no LDS, no waits)
@@ -190,18 +229,12 @@ template <bool BLOCK, int N> __device__ __forceinline__ void row_sums(float (&v)
         turn ^= 1;
     }
 }
-// sum over one piece of what lies inside the row
-template <int V, bool TAIL> __device__ __forceinline__ float piece_sum(const float* v, int left) {
+// sum over one piece of what lies inside the row.  TAIL: keep[e] = all ones inside the row, 0 behind it; not needed where the values behind it are zeros.
+template <int V, bool TAIL, bool ZEROS> __device__ __forceinline__ float piece_sum(const float* v, int left, const unsigned* keep) {
     float s = 0.f;
-    if constexpr (!TAIL) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += v[e];
-        return left > 0 ? s : 0.f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) s += e < left ? v[e] : 0.f;
-        return s;
-    }
+    for (int e = 0; e < V; ++e) s += TAIL && !ZEROS ? __uint_as_float(__float_as_uint(v[e]) & keep[e]) : v[e];
+    return TAIL || left > 0 ? s : 0.f;
 }
 
 // 1 / (1 + exp(-g)) on the hardware's 2^x and reciprocal (1 step each); the rounding of g log2(e) is carried along, or it would cost |g| steps
@@ -246,6 +279,7 @@ inline Shape shape_of(const codeps_channel_norm_desc* d) {
 }
 // Blocks work on rows of one item (the rows that share an ITEM gate; all rows otherwise): block (item, slice) takes every slices-th group of rows, so that the
 // chip walks through memory in step (contiguous ranges per block: the stride-4 norm's backward pass 98 instead of 77 us).  Blocks loop over items.
+inline bool shared_lines(const codeps_channel_norm_desc* d) { return d->channels * (d->x_type == CODEPS_F32 ? 4 : 2) % 128 != 0; }
 struct Plan { Shape s; int items, rpi, slices, blocks; };
 inline Plan plan_of(const codeps_channel_norm_desc* d, int want, int resident) {
     Plan p;
@@ -255,6 +289,7 @@ inline Plan plan_of(const codeps_channel_norm_desc* d, int want, int resident) {
     p.items = per_item ? std::max(1, (int)(d->rows / d->rows_per_item)) : 1;
     const int most = (int)std::max<long long>(1, ((long long)p.rpi + p.s.rpb - 1) / p.s.rpb);
     p.slices = std::max(1, std::min(most, want / p.items));
+    if (p.slices > 8 && shared_lines(d)) p.slices &= ~7;                       // (whole rounds over the XCDs: slice_of)
     p.blocks = std::min(p.items, std::max(1, resident / p.slices)) * p.slices;
     return p;
 }
@@ -290,6 +325,7 @@ inline Args args_of(const codeps_channel_norm_desc* d, const Plan& p) {
     a.kind = d->kind; a.next = d->next_kind; a.act = d->gate_act;
     a.wt = d->weight_type; a.gt = d->gate_type; a.nt = d->next_weight_type;
     a.scale = d->scale; a.eps = d->eps; a.neps = d->next_eps; a.inv_c = (float)(1.0 / d->channels);
+    a.shared_lines = shared_lines(d);
     a.lpr_log2 = p.s.lpr_log2; a.items = p.items; a.rpi = p.rpi; a.slices = p.slices;
     if (d->gate_mode == CODEPS_GATE_CHANNEL) a.gp = 0;                          // (the one item's row)
     return a;

@@ -47,6 +47,7 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
     // this lane's row behind the wave's first, in elements
     const int ox = sub * (int)a.xp, orr = sub * (int)a.rp, og = sub * (int)a.gp, ody = sub * (int)a.dyp, odh = sub * (int)a.dhp, oc = sub * C;
     int c0[NCH], left[NCH];
+    unsigned keep[TAIL && FULL ? E : 1];
     float w[E], b[FULL ? E : 1], nw[FULL ? E : 1];
     float gv[HELD ? E : 1], gs[HELD ? E : 1];                                     // alpha act(g), alpha act'(g) of the item
     float aw[SUMS ? E : 1], ab[SUMS ? E : 1], anw[SUMS && FULL ? E : 1], anb[SUMS && FULL ? E : 1], ag[SUMS && HELD ? E : 1];
@@ -54,6 +55,10 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
     for (int j = 0; j < NCH; ++j) {
         c0[j] = (j * at_.lpr + lane) * V;
         left[j] = C - c0[j];
+        if constexpr (TAIL && FULL) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) keep[j * V + e] = e < left[j] ? ~0u : 0u;
+        }
         load_vector<V>(a.w, a.wt, 0, c0[j], C, 1.f, w + j * V);
         if constexpr (FULL) {
             load_vector<V>(a.b, a.wt, 0, c0[j], C, 0.f, b + j * V);
@@ -67,7 +72,7 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
             if constexpr (FULL) anw[k] = anb[k] = 0.f;
         }
     }
-    const int S = a.slices, slice = (int)(blockIdx.x % (unsigned)S);
+    const int S = a.slices, slice = slice_of(blockIdx.x, S, a.shared_lines);
     const bool has_r = a.r != nullptr;
     for (unsigned item = blockIdx.x / (unsigned)S; item < (unsigned)a.items; item += gridDim.x / (unsigned)S) {
         if constexpr (HELD) {
@@ -149,8 +154,8 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
                             q[e] *= nw[k];
                             t[k] *= nw[k];
                         }
-                        s[0] += piece_sum<V, TAIL>(t + j * V, left[j]);
-                        s[1] += piece_sum<V, TAIL>(q, left[j]);
+                        s[0] += piece_sum<V, TAIL, true>(t + j * V, left[j], keep);        // (dh is 0 behind the row's end)
+                        s[1] += piece_sum<V, TAIL, true>(q, left[j], keep);
                     }
                     row_sums<BLOCK>(s, lpr_log2, red, turn);
                     s[0] = a.next == CODEPS_NORM_LAYER ? s[0] * a.inv_c : 0.f;
@@ -193,8 +198,8 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
                     q[e] *= w[k];
                     d[k] *= w[k];
                 }
-                s[0] += piece_sum<V, TAIL>(d + j * V, left[j]);
-                s[1] += piece_sum<V, TAIL>(q, left[j]);
+                s[0] += piece_sum<V, TAIL, !FULL>(d + j * V, left[j], keep + (TAIL && FULL ? j * V : 0));
+                s[1] += piece_sum<V, TAIL, !FULL>(q, left[j], keep + (TAIL && FULL ? j * V : 0));
             }
             if (a.kind) {
                 row_sums<BLOCK>(s, lpr_log2, red, turn);
@@ -229,7 +234,7 @@ template <typename TX, typename TR, bool TAIL, bool FULL, int GATE>
 __global__ __launch_bounds__(256) void channel_norm_columns_kernel(Args a) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8;
     constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS;
-    const int C = a.C, S = a.slices, slice = (int)(blockIdx.x % (unsigned)S), c0 = (int)(blockIdx.y * 256 + threadIdx.x) * V;
+    const int C = a.C, S = a.slices, slice = slice_of(blockIdx.x, S, a.shared_lines), c0 = (int)(blockIdx.y * 256 + threadIdx.x) * V;
     float w[V], b[V], nw[V], gv[V], gs[V], aw[V] = {}, ab[V] = {}, anw[V] = {}, anb[V] = {}, ag[V];
     load_vector<V>(a.w, a.wt, 0, c0, C, 1.f, w);
     load_vector<V>(a.b, a.wt, 0, c0, C, 0.f, b);

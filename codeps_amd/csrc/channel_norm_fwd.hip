@@ -5,15 +5,15 @@ namespace {
 
 // mean and 1 / deviation of the row that v holds.  The deviations are summed around the mean, in a second sweep over registers: the difference of two
 // large sums would lose them where the mean is large.
-template <int V, int NCH, bool BLOCK, bool TAIL>
-__device__ __forceinline__ void row_stats(const float* v, const int* left, int kind, float eps, float inv_c, int lpr_log2, float (*red)[32], int& turn,
+template <int V, int NCH, bool BLOCK, bool TAIL, bool ZEROS>
+__device__ __forceinline__ void row_stats(const float* v, const int* left, const unsigned* keep, int kind, float eps, float inv_c, int lpr_log2, float (*red)[32], int& turn,
                                           float& mu, float& rho) {
     float s[1];
     mu = 0.f;
     if (kind == CODEPS_NORM_LAYER) {
         s[0] = 0.f;
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) s[0] += piece_sum<V, TAIL>(v + j * V, left[j]);
+        for (int j = 0; j < NCH; ++j) s[0] += piece_sum<V, TAIL, ZEROS>(v + j * V, left[j], keep + (TAIL ? j * V : 0));
         row_sums<BLOCK>(s, lpr_log2, red, turn);
         mu = s[0] * inv_c;
     }
@@ -23,7 +23,7 @@ __device__ __forceinline__ void row_stats(const float* v, const int* left, int k
         float q[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) { const float t = v[j * V + e] - mu; q[e] = t * t; }
-        s[0] += piece_sum<V, TAIL>(q, left[j]);
+        s[0] += piece_sum<V, TAIL, false>(q, left[j], keep + (TAIL ? j * V : 0));
     }
     row_sums<BLOCK>(s, lpr_log2, red, turn);
     rho = 1.f / sqrtf(s[0] * inv_c + eps);
@@ -39,11 +39,16 @@ __global__ __launch_bounds__(BLOCK ? 1024 : WAVE_THREADS) void channel_norm_fwd_
     const int lpr = at_.lpr, lane = at_.lane, sub = at_.sub;
     const int ox = sub * (int)a.xp, orr = sub * (int)a.rp, og = sub * (int)a.gp, oc = sub * C;        // this lane's row behind the wave's first, in elements
     int c0[NCH], left[NCH];
+    unsigned keep[TAIL ? E : 1];
     float w[E], b[E], nw[FULL ? E : 1], nb[FULL ? E : 1], g[FULL && GATE != GATE_NONE ? E : 1];     // the vectors stay in registers over the rows of a block
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         c0[j] = (j * lpr + lane) * V;
         left[j] = C - c0[j];
+        if constexpr (TAIL) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) keep[j * V + e] = e < left[j] ? ~0u : 0u;
+        }
         load_vector<V>(a.w, a.wt, 0, c0[j], C, 1.f, w + j * V);
         load_vector<V>(a.b, a.wt, 0, c0[j], C, 0.f, b + j * V);
         if constexpr (FULL) {
@@ -51,7 +56,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : WAVE_THREADS) void channel_norm_fwd_
             load_vector<V>(a.nb, a.nt, 0, c0[j], C, 0.f, nb + j * V);
         }
     }
-    const int S = a.slices, slice = (int)(blockIdx.x % (unsigned)S);
+    const int S = a.slices, slice = slice_of(blockIdx.x, S, a.shared_lines);
     const bool has_r = a.r != nullptr;
     for (unsigned item = blockIdx.x / (unsigned)S; item < (unsigned)a.items; item += gridDim.x / (unsigned)S) {
         if constexpr (FULL && GATE == GATE_HELD) {
@@ -79,7 +84,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : WAVE_THREADS) void channel_norm_fwd_
                 }
             }
             float mu = 0.f, rho = 1.f, nmu = 0.f, nrho = 1.f;
-            if (a.kind) row_stats<V, NCH, BLOCK, TAIL>(v, left, a.kind, a.eps, a.inv_c, lpr_log2, red, turn, mu, rho);
+            if (a.kind) row_stats<V, NCH, BLOCK, TAIL, true>(v, left, keep, a.kind, a.eps, a.inv_c, lpr_log2, red, turn, mu, rho);
 #pragma unroll
             for (int k = 0; k < E; ++k) v[k] = (v[k] - mu) * rho * w[k] + b[k];
             if constexpr (!FULL) {
@@ -95,7 +100,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : WAVE_THREADS) void channel_norm_fwd_
 #pragma unroll
                 for (int j = 0; j < NCH; ++j) store_piece<V, TAIL>((TR*)a.y + row * C, oc, c0[j], C, v + j * V);
                 if (a.next) {
-                    row_stats<V, NCH, BLOCK, TAIL>(v, left, a.next, a.neps, a.inv_c, lpr_log2, red, turn, nmu, nrho);
+                    row_stats<V, NCH, BLOCK, TAIL, false>(v, left, keep, a.next, a.neps, a.inv_c, lpr_log2, red, turn, nmu, nrho);
 #pragma unroll
                     for (int k = 0; k < E; ++k) v[k] = (v[k] - nmu) * nrho * nw[k] + nb[k];
 #pragma unroll
