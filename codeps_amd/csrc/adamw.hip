@@ -276,6 +276,15 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
 // ------------------------------------------------------------------------------------------------------------------------ the update
 struct States { float *m, *v; unsigned char *mc, *me, *rc, *re; };
 
+// The new moments in 64 bits, every operation rounded by itself: 16-bit gradients and codes lie on coarse grids, sums fall exactly on borders between codes,
+// and there the last bit decides.
+__device__ __forceinline__ void moments64(const Factors& f, double m0, double r0, double g, double& m, double& v) {
+#pragma clang fp contract(off)
+    const double gg = g * f.gs, a = f.b1 * m0, b = f.ob1 * gg, c = f.b2 * (r0 * r0), d = f.ob2 * gg * gg;
+    m = a + b;
+    v = c + d;
+}
+
 // one chunk of a tensor; WIDE: 32-bit states.  The gradients are loaded last: their type is known at run time, and where the branches meet the compiler waits.
 template <bool WIDE, bool TAIL>
 __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, const void* gp, int gt, float* const ema, long long start, const States& st, float al, float oal) {
@@ -346,16 +355,16 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
                 const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(c[e]);
                 const int low = place_of<MANT_M>(am, nm);
-                const unsigned slack = 2u + (unsigned)fminf(__builtin_ldexpf(size, 143 + MANT_M - 22 - nm - low), 32000.f);
+                const unsigned slack = 2u + (unsigned)fminf(__builtin_ldexpf(size, 143 + MANT_M - 22 - nm - low), 33000.f);        // (2 * 33002 covers every remainder)
                 bool minus = a[k][e] < 0.f;
                 unsigned cm = encode<MANT_M>(am, nm, low, rnd & 0xffffu, slack, dm);
                 unsigned cr = encode<MANT_R>(b[k][e], nr, place_of<MANT_R>(b[k][e], nr), rnd >> 16, 2u, dr);
                 if (dm || dr || small) {
-                    const double gg = (double)g[k][e] * f.gs;
-                    const double m = f.b1 * (double)m0[e] + f.ob1 * gg;
+                    double m, v;
+                    moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m, v);
                     minus = m < 0.0;
                     cm = encode64<MANT_M>(fabs(m), nm, rnd & 0xffffu);
-                    cr = encode64<MANT_R>(sqrt(f.b2 * ((double)r0[e] * (double)r0[e]) + f.ob2 * gg * gg), nr, rnd >> 16);
+                    cr = encode64<MANT_R>(sqrt(v), nr, rnd >> 16);
                 }
                 ncm |= (cm | (minus ? 128u : 0u)) << (8 * e);
                 ncr |= cr << (8 * e);

@@ -5,6 +5,7 @@ all arithmetic happens in libcodeps_hip.so.  Every function raises on CPU tensor
 """
 import array
 import ctypes
+import operator
 import os
 import weakref
 
@@ -2596,9 +2597,12 @@ def _dense(t):
     return True
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _types_of(tensors, device):
     """Element types of a list of tensors as the C ABI's bytes; raises unless all are fp32, bf16 or fp16 on `device`."""
-    dtypes = {t.dtype for t in tensors}
+    dtypes = set(map(_dtype_of, tensors))
     if not dtypes <= _TYPES.keys() or set(map(torch.Tensor.get_device, tensors)) - {device.index}:
         raise CodepsHipError(f"gradients are fp32, bf16 or fp16 tensors on {device}: got {sorted({(str(t.dtype), str(t.device)) for t in tensors})}")
     return bytes([_TYPES[dtypes.pop()]]) * len(tensors) if len(dtypes) == 1 else bytes([_TYPES[t.dtype] for t in tensors])
@@ -2607,7 +2611,12 @@ def _types_of(tensors, device):
 def grad_norm(grads, scale=1.0):
     """|scale g|_2 over a list of gradients (None entries are skipped), fp32 on the device: what AdamW clips by (C ABI: codeps_grad_norm).  fp32, bf16 and
     fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow."""
-    grads = [g for g in grads if g is not None]
+    grads = list(grads)
+    try:
+        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+    except TypeError:                                 # (a None among them)
+        grads = [g for g in grads if g is not None]
+        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
     n = len(grads)
     if n == 0:
         raise CodepsHipError("grad_norm: no gradients")
@@ -2616,7 +2625,8 @@ def grad_norm(grads, scale=1.0):
     types = _types_of(grads, dev)
     if not all(map(torch.Tensor.is_contiguous, grads)):
         grads = [g if _dense(g) else g.contiguous() for g in grads]
-    ptrs, numels = array.array("Q", map(torch.Tensor.data_ptr, grads)), array.array("q", map(torch.Tensor.numel, grads))
+        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+    numels = array.array("q", map(torch.Tensor.numel, grads))
     out = torch.empty((), dtype=torch.float32, device=dev)
     nbytes = lib().codeps_grad_norm_workspace_bytes(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
