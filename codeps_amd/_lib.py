@@ -20,6 +20,7 @@ DIAG_LIB_PATH = os.path.join(_HERE, "libcodeps_diag.so")
 
 _lib = None
 _diag = None
+_bind = None
 
 
 class CodepsHipError(RuntimeError):
@@ -285,6 +286,22 @@ def diag_lib():
             _sig(getattr(handle, name), res, *args)
         _diag = handle
     return _diag
+
+
+def bind():
+    """codeps_amd._bind (csrc/bind.cpp): the training-step operators' tensor handling and autograd nodes, bound to the library of lib()."""
+    global _bind
+    if _bind is None:
+        handle = lib()
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise CodepsHipError(f"codeps_amd/_bind.so cannot be loaded ({e}): build it with `make -C codeps_amd/csrc`") from e
+        module.init(CodepsHipError, torch.OutOfMemoryError, *[ctypes.cast(getattr(handle, name), c_void_p).value for name in
+                                      ("codeps_last_error", "codeps_channel_norm_fwd", "codeps_channel_norm_bwd_workspace_bytes", "codeps_channel_norm_bwd",
+                                       "codeps_grad_norm_workspace_bytes", "codeps_grad_norm")])
+        _bind = module
+    return _bind
 
 
 def check(rc, what):

@@ -3,16 +3,14 @@
 PyTorch supplies device memory (caching allocator), the current HIP stream and the autograd tape;
 all arithmetic happens in libcodeps_hip.so.  Every function raises on CPU tensors -- no fallback.
 """
-import array
 import ctypes
-import operator
 import os
 import weakref
 
 import torch
 
 from . import _lib
-from ._lib import CodepsHipError, check, lib, ptr, require_cuda, stream_ptr
+from ._lib import CodepsHipError, bind, check, lib, ptr, require_cuda, stream_ptr
 
 _seed_counter = [0x5EED]
 _noise_counter = [None]       # device uint64 step counter mixed into the photometric tie-break seed (set by the step harness)
@@ -2345,195 +2343,28 @@ def weighted_sum(losses, weights, factors=None, denom=None):
 
 
 # ---------------------------------------------------------------------------------------- channel norms (C ABI: codeps_channel_norm_*)
+# Checks, layouts and the autograd node are in csrc/bind.cpp.  64 rows x 9 channels, forward alone / forward and backward, per call: 8.3 / 103 us through
+# ctypes and a torch.autograd.Function, 4.7 / 69 us through it (an autograd.Function that launches nothing costs 62 us on the same box).
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 _GATE_ACTS = {None: 0, "sigmoid": 1, "silu": 2}
-_MAX_NORM_CHANNELS = 8192
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream          # (device index) -> hipStream_t; torch.cuda.current_stream builds an object (4 us)
-
-
-def _on_device(device):
-    """A context that makes `device` the current one for launches, None when it is already (torch.cuda.device costs microseconds)."""
-    return None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
-
-
-def _launch(device, what, call, *args):
-    """check(call(*args, stream)) on the current stream of `device`."""
-    scope = _on_device(device)
-    if scope is None:
-        rc = call(*args, _raw_stream(device.index))
-    else:
-        with scope:
-            rc = call(*args, _raw_stream(device.index))
-    if rc != 0:
-        check(rc, what)
-
-
-def _at(t):
-    return None if t is None else t.data_ptr()
-
-
-def _pitched(t):
-    """(tensor, elements from row to row): t itself when its channels are dense and its rows lie at one distance, else a contiguous copy."""
-    c = t.shape[-1]
-    if t.is_contiguous():
-        return t, c
-    if t.stride(-1) == 1 or c == 1:
-        pitch, span = None, 1
-        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-            if size == 1:
-                continue
-            if pitch is None:
-                pitch = stride
-            elif stride != pitch * span:
-                pitch = -1
-                break
-            span *= size
-        if pitch is None:
-            return t, c
-        if c <= pitch < 1 << 24:
-            return t, pitch
-    return t.contiguous(), c
-
-
-def _vector(v, c, what, device):
-    if v is None:
+def _sinks(*vectors):
+    """The vectors' flat-gradient views, None where there is none (register_grad_sink), or None when nothing is registered."""
+    if not _grad_sink:
         return None
-    if v.dim() != 1 or v.shape[0] != c or v.dtype not in _TYPES or v.device != device:
-        raise CodepsHipError(f"{what}: one value per channel ({c}) in fp32, bf16 or fp16 on {device}, got {tuple(v.shape)} {v.dtype} on {v.device}")
-    return v.contiguous()
-
-
-def _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, want_stats):
-    """One forward launch.  cfg = (full, kind, eps, gate mode, gate activation, rows per item, scale, next kind, next eps)."""
-    full, kind, eps, mode, act, per_item, scale, nkind, neps = cfg
-    c = x.shape[-1]
-    rows = x.numel() // c
-    xr, xp = _pitched(x)
-    xt = rt = _TYPES[x.dtype]
-    rr, rp, gr, gp, gt = None, c, None, c, 0
-    if residual is not None:
-        rr, rp = _pitched(residual)
-        rt = _TYPES[residual.dtype]
-    if gate is not None:
-        gr, gp = _pitched(gate)
-        gt = _TYPES[gate.dtype]
-    vec, nvec = weight if weight is not None else bias, next_weight if next_weight is not None else next_bias
-    d = _lib.ChannelNormDesc(rows, xp, rp, gp, c, c, c, per_item, full, kind, nkind, mode, act, xt, rt, 0 if vec is None else _TYPES[vec.dtype], gt,
-                             0 if nvec is None else _TYPES[nvec.dtype], scale, eps, neps)
-    y = (x if residual is None else residual).new_empty(x.shape) if full else None
-    h = x.new_empty(x.shape) if (nkind or not full) else None
-    stats = torch.empty((rows, 4 if full else 2), dtype=torch.float32, device=x.device) if want_stats else None
-    _launch(x.device, "codeps_channel_norm_fwd", lib().codeps_channel_norm_fwd, ctypes.byref(d), xr.data_ptr(), _at(rr), _at(gr), _at(weight), _at(bias),
-            _at(next_weight), _at(next_bias), _at(y), _at(h), _at(stats))
-    return y, h, stats, d, xr, rr, gr
-
-
-class _ChannelNorm(torch.autograd.Function):
-    """Both public forms with gradients (cfg: _channel_norm_fwd)."""
-
-    @staticmethod
-    def forward(ctx, x, residual, gate, weight, bias, next_weight, next_bias, cfg):
-        y, h, stats, d, xr, rr, gr = _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, True)
-        ctx.save_for_backward(xr, rr if d.next_kind else None, gr, weight, bias, next_weight, stats)
-        ctx.d, ctx.gate_shape, ctx.res_dtype = d, None if gate is None else gate.shape, None if residual is None else residual.dtype
-        vectors = (weight, bias, next_weight, next_bias)
-        ctx.vec_dtypes = [None if v is None else v.dtype for v in vectors]
-        ctx.sinks = [grad_sink(v) if v is not None and v.requires_grad else None for v in vectors]     # (flat-gradient views: fp32, contiguous)
-        ctx.set_materialize_grads(False)
-        if not d.full:
-            return h
-        return (y, h) if d.next_kind else y
-
-    @staticmethod
-    def backward(ctx, *douts):
-        if torch.is_grad_enabled():                   # (create_graph: a second derivative raises instead of being silently zero)
-            return _channel_norm_bwd_once(ctx, *douts)
-        return _channel_norm_bwd(ctx, *douts)
-
-
-def _channel_norm_bwd(ctx, *douts):
-    x, residual, gate, weight, bias, next_weight, stats = ctx.saved_tensors
-    d = _lib.ChannelNormDesc.from_buffer_copy(ctx.d)  # (two backward passes of one forward may run at once)
-    c, dev, need, sinks = d.channels, x.device, ctx.needs_input_grad, ctx.sinks
-    dy, dh = (douts[0], douts[1] if d.next_kind else None) if d.full else (None, douts[0])
-    if dy is None and dh is None:
-        return (None,) * 8
-    if dy is not None:
-        dy, d.dy_pitch = _pitched(dy)
-    if dh is not None:
-        dh, d.dh_pitch = _pitched(dh)
-    elif d.next_kind:                                 # h is not part of the loss: the block's end alone
-        d.next_kind = 0
-        residual = None
-    dx = x.new_empty(x.shape) if need[0] else None
-    # without a next norm y's gradient is the residual's: handed on, not copied
-    dres = torch.empty(x.shape, dtype=ctx.res_dtype, device=dev) if need[1] and d.next_kind else None
-    dgate = (gate.new_empty if d.rows else gate.new_zeros)(ctx.gate_shape) if need[2] else None
-    outs, acc = [None] * 4, 0
-    for i in range(4 if d.next_kind else 2):
-        if need[3 + i]:
-            if sinks[i] is not None:
-                outs[i], acc = sinks[i], acc | 1 << i
-            else:
-                outs[i] = torch.empty(c, dtype=ctx.vec_dtypes[i], device=dev)
-    nbytes = lib().codeps_channel_norm_bwd_workspace_bytes(ctypes.byref(d))
-    if nbytes == 0:
-        check(-1, "codeps_channel_norm_bwd_workspace_bytes")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)              # not a cached one: captured graphs must not share it
-    _launch(dev, "codeps_channel_norm_bwd", lib().codeps_channel_norm_bwd, ctypes.byref(d), x.data_ptr(), _at(residual), _at(gate), _at(weight), _at(bias),
-            _at(next_weight), stats.data_ptr(), _at(dy), _at(dh), _at(dx), _at(dres), _at(dgate), _at(outs[0]), _at(outs[1]), _at(outs[2]), _at(outs[3]),
-            acc, ws.data_ptr(), nbytes)
-    outs = [None if sinks[i] is not None else outs[i] for i in range(4)]
-    return (dx, dres if d.next_kind or not need[1] else douts[0], dgate, *outs, None)
-
-
-_channel_norm_bwd_once = torch.autograd.function.once_differentiable(_channel_norm_bwd)
-
-
-def _channel_norm_apply(x, residual, gate, weight, bias, next_weight, next_bias, cfg):
-    if torch.is_grad_enabled():
-        for t in (x, residual, gate, weight, bias, next_weight, next_bias):
-            if t is not None and t.requires_grad:
-                return _ChannelNorm.apply(x, residual, gate, weight, bias, next_weight, next_bias, cfg)
-    y, h = _channel_norm_fwd(x, residual, gate, weight, bias, next_weight, next_bias, cfg, False)[:2]
-    if not cfg[0]:
-        return h
-    return (y, h) if cfg[7] else y
-
-
-def _check_rows(x, what):
-    require_cuda(x)
-    if x.dtype not in _TYPES:
-        raise CodepsHipError(f"{what}: fp32, bf16 or fp16, got {x.dtype}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MAX_NORM_CHANNELS:
-        raise CodepsHipError(f"{what}: [..., channels] with 1 .. {_MAX_NORM_CHANNELS} channels, got {tuple(x.shape)}")
-    return x.shape[-1]
-
-
-def _check_norm(kind, weight, bias, eps, c, what, device):
-    if kind not in _NORM_KINDS:
-        raise CodepsHipError(f"{what}: kind is \"layer\", \"rms\" or None, got {kind!r}")
-    if not eps >= 0.0:
-        raise CodepsHipError(f"{what}: eps = {eps}")
-    weight, bias = _vector(weight, c, what + ": weight", device), _vector(bias, c, what + ": bias", device)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise CodepsHipError(f"{what}: weight ({weight.dtype}) and bias ({bias.dtype}) have one type")
-    return weight, bias
+    return tuple(grad_sink(v) if v is not None and v.requires_grad else None for v in vectors)
 
 
 def channel_norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
     """Norm over the last dimension of x [..., C], the channels of a pixel (NHWC) or token:  n(x) weight + bias  with
     n(x) = (x - mean) / sqrt(var + eps)  ("layer")  or  x / sqrt(mean x^2 + eps)  ("rms").  fp32, bf16 or fp16; the statistics are fp32.  weight, bias
     [C]: one type of the three, their gradients are summed in fp32 in a fixed order.  x may be a channel slice of a wider (padded) map: rows are read
-    where they lie.  Unlike F.batch_norm_train it does not depend on the other items of the batch."""
-    c = _check_rows(x, "channel_norm")
-    if kind is None:
-        raise CodepsHipError("channel_norm: kind is \"layer\" or \"rms\"")
-    weight, bias = _check_norm(kind, weight, bias, eps, c, "channel_norm", x.device)
-    return _channel_norm_apply(x, None, None, weight, bias, None, None, (0, _NORM_KINDS[kind], eps, 0, 0, 1, 1.0, 0, 0.0))
+    where they lie.  1 <= C <= 8192.  Unlike F.batch_norm_train it does not depend on the other items of the batch."""
+    if kind != "layer" and kind != "rms":
+        raise CodepsHipError(f"channel_norm: kind is \"layer\" or \"rms\", got {kind!r}")
+    return bind().channel_norm(x, weight, bias, _NORM_KINDS[kind], eps, _sinks(weight, bias, None, None))
 
 
 def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=None, gate_act=None, scale=1.0, next_kind=None,
@@ -2542,36 +2373,14 @@ def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="lay
         y = residual + scale act(gate) (n(x) weight + bias),   h = n'(y) next_weight + next_bias
     Returns y, or (y, h) with next_kind.  x [..., C] is the block's output; kind None leaves it as it is (times weight, plus bias, if given).
     residual: x's shape, x's type or fp32 (a residual stream in 32 bits around 16-bit blocks); y has its type, h has x's.  None: zeros.
-    gate: [C] (layer scale), one row per item of the first dimension ([B, C], or x's number of dimensions with ones in between), or x's shape;
+    gate: [C] (layer scale), one row per item of the first dimension ([B, C], or x's number of dimensions with ones in between), or x's shape (and type);
     gate_act: None, "sigmoid" or "silu".  scale: a float.  h is the norm of y before y is rounded to its type."""
-    what = "channel_norm_residual"
-    c = _check_rows(x, what)
-    weight, bias = _check_norm(kind, weight, bias, eps, c, what, x.device)
-    next_weight, next_bias = _check_norm(next_kind, next_weight, next_bias, next_eps, c, what + " (next)", x.device)
-    if next_kind is None and (next_weight is not None or next_bias is not None):
-        raise CodepsHipError(f"{what}: next_weight / next_bias without next_kind")
-    if residual is not None:
-        if residual.shape != x.shape or residual.device != x.device or residual.dtype not in (x.dtype, torch.float32):
-            raise CodepsHipError(f"{what}: residual has x's shape and device, and x's type or fp32: got {tuple(residual.shape)} {residual.dtype} on "
-                                 f"{residual.device} for {tuple(x.shape)} {x.dtype} on {x.device}")
-    if gate_act not in _GATE_ACTS or (gate is None and gate_act is not None):
-        raise CodepsHipError(f"{what}: gate_act is None, \"sigmoid\" or \"silu\", and goes with a gate: got {gate_act!r}")
-    mode, per_item = 0, 1
-    if gate is not None:
-        if gate.dtype not in _TYPES or gate.device != x.device or gate.dim() < 1 or gate.shape[-1] != c:
-            raise CodepsHipError(f"{what}: gate [..., {c}] in fp32, bf16 or fp16 on {x.device}, got {tuple(gate.shape)} {gate.dtype} on {gate.device}")
-        if gate.dim() == 1:
-            mode = 1
-        elif gate.shape == x.shape:
-            mode = 3
-            if gate.dtype != x.dtype:
-                raise CodepsHipError(f"{what}: a gate of x's shape has x's type, got {gate.dtype} for {x.dtype}")
-        elif (gate.dim() == 2 or gate.dim() == x.dim()) and gate.shape[0] == x.shape[0] and gate.numel() == gate.shape[0] * c and x.dim() > 2:
-            mode, per_item = 2, max(1, x.numel() // c // max(1, x.shape[0]))
-        else:
-            raise CodepsHipError(f"{what}: gate is [{c}], one row per item of x's first dimension, or x's shape: got {tuple(gate.shape)} for {tuple(x.shape)}")
-    return _channel_norm_apply(x, residual, gate, weight, bias, next_weight, next_bias,
-                               (1, _NORM_KINDS[kind], eps, mode, _GATE_ACTS[gate_act], per_item, float(scale), _NORM_KINDS[next_kind], next_eps))
+    if kind not in _NORM_KINDS or next_kind not in _NORM_KINDS:
+        raise CodepsHipError(f"channel_norm_residual: kind and next_kind are \"layer\", \"rms\" or None, got {kind!r} and {next_kind!r}")
+    if gate_act not in _GATE_ACTS:
+        raise CodepsHipError(f"channel_norm_residual: gate_act is None, \"sigmoid\" or \"silu\", got {gate_act!r}")
+    return bind().channel_norm_residual(x, residual, weight, bias, _NORM_KINDS[kind], eps, gate, _GATE_ACTS[gate_act], scale, _NORM_KINDS[next_kind],
+                                        next_weight, next_bias, next_eps, _sinks(weight, bias, next_weight, next_bias))
 
 
 # ---------------------------------------------------------------------------------------- optimiser
@@ -2585,54 +2394,10 @@ def adam_ema_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-4, betas=(0.9,
     invalidate_weight_cache()
 
 
-def _dense(t):
-    """Whether t's elements fill one stretch of memory, in any order of its dimensions (contiguous, channels-last, ...)."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-_dtype_of = operator.attrgetter("dtype")
-
-
-def _types_of(tensors, device):
-    """Element types of a list of tensors as the C ABI's bytes; raises unless all are fp32, bf16 or fp16 on `device`."""
-    dtypes = set(map(_dtype_of, tensors))
-    if not dtypes <= _TYPES.keys() or set(map(torch.Tensor.get_device, tensors)) - {device.index}:
-        raise CodepsHipError(f"gradients are fp32, bf16 or fp16 tensors on {device}: got {sorted({(str(t.dtype), str(t.device)) for t in tensors})}")
-    return bytes([_TYPES[dtypes.pop()]]) * len(tensors) if len(dtypes) == 1 else bytes([_TYPES[t.dtype] for t in tensors])
-
-
 def grad_norm(grads, scale=1.0):
     """|scale g|_2 over a list of gradients (None entries are skipped), fp32 on the device: what AdamW clips by (C ABI: codeps_grad_norm).  fp32, bf16 and
     fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow."""
-    grads = list(grads)
-    try:
-        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
-    except TypeError:                                 # (a None among them)
-        grads = [g for g in grads if g is not None]
-        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
-    n = len(grads)
-    if n == 0:
-        raise CodepsHipError("grad_norm: no gradients")
-    dev = grads[0].device
-    require_cuda(grads[0])
-    types = _types_of(grads, dev)
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
-        ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
-    numels = array.array("q", map(torch.Tensor.numel, grads))
-    out = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = lib().codeps_grad_norm_workspace_bytes(n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch(dev, "codeps_grad_norm", lib().codeps_grad_norm, ptrs.buffer_info()[0], types, numels.buffer_info()[0], n, float(scale), out.data_ptr(),
-            ws.data_ptr(), nbytes)
-    return out
+    return bind().grad_norm(grads, scale)
 
 
 # ---------------------------------------------------------------------------------------- panoptic fusion

@@ -13,11 +13,39 @@ import ctypes
 import torch
 
 from . import functional as F
-from ._lib import AdamWGroup, CodepsHipError, lib, ptr, require_cuda
+from ._lib import AdamWGroup, CodepsHipError, bind, check, lib, ptr, require_cuda
 
 BLOCK = 256                     # elements of one tensor that share an exponent byte
 CHUNK = 2048                    # elements of one tensor that a work group updates
 MAX_GROUPS = 16
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream          # (device index) -> hipStream_t; torch.cuda.current_stream builds an object (4 us)
+
+
+def _launch(device, what, call, *args):
+    """check(call(*args, stream)) on the current stream of `device`, which need not be the current device."""
+    if device.index == torch._C._cuda_getDevice():
+        check(call(*args, _raw_stream(device.index)), what)
+    else:
+        with torch.cuda.device(device):
+            check(call(*args, _raw_stream(device.index)), what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, in any order of its dimensions (contiguous, channels-last, ...)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
 
 
 def _same_layout(a, b):
@@ -68,7 +96,7 @@ class AdamW:
             require_cuda(p)
             if p.dtype != torch.float32 or p.device != dev:
                 raise CodepsHipError(f"AdamW: fp32 parameters on one device, got {p.dtype} on {p.device} (16-bit weights: `copies` of fp32 ones)")
-            if not F._dense(p):
+            if not _dense(p):
                 raise CodepsHipError(f"AdamW: a parameter of shape {tuple(p.shape)} with strides {p.stride()} is not dense")
             if p.numel() and p.data_ptr() in seen:
                 raise CodepsHipError("AdamW: a parameter is listed twice")
@@ -125,7 +153,7 @@ class AdamW:
         return tensors
 
     def _addresses(self):
-        return list(map(torch.Tensor.data_ptr, self.params))
+        return array.array("Q", [t.data_ptr() for t in self.params]).tobytes()
 
     def _fill_items(self):
         """(Re)writes the device table in place: a captured step reads the same table."""
@@ -150,38 +178,25 @@ class AdamW:
             elif p.grad is not None:
                 p.grad.zero_()
 
-    @torch.no_grad()
     def step(self, grads=None, *, grad_scale=1.0, apply_ema=True):
         """One update of every parameter that has a gradient.  grads: one tensor (or None) per parameter in the order of `params`; default: their .grad.
         The others keep value, states and step count.  grad_scale multiplies the gradients (1 / world size after a summing all-reduce); apply_ema False
         leaves the EMA tensors alone."""
         params = self.params
         grads = [p.grad for p in params] if grads is None else grads
-        if len(grads) != len(params):
-            raise CodepsHipError(f"AdamW.step: one gradient (or None) per parameter ({len(params)}), got {len(grads)}")
-        some = [g for g in grads if g is not None]
-        whole = len(some) == len(params)
-        shapes = self._shapes if whole else [s for s, g in zip(self._shapes, grads) if g is not None]
-        if [g.shape for g in some] != shapes:
-            raise CodepsHipError("AdamW.step: gradients have their parameter's shape")
-        types = F._types_of(some, self.device)
-        if not (all(map(torch.Tensor.is_contiguous, some)) and all(map(torch.Tensor.is_contiguous, params))):
-            if any(p.numel() != k or not F._dense(p) for p, k in zip(params, self._numels)):
+        ptrs, types, moved, mixed = bind().optimizer_lists(params, grads, self._table_addresses)
+        if mixed:
+            if any(p.numel() != k or not _dense(p) for p, k in zip(params, self._numels)):
                 raise CodepsHipError("AdamW.step: a parameter has changed its shape or layout since it was listed")
-            grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
-            some = [g for g in grads if g is not None]
-        if self._addresses() != self._table_addresses:
-            if [p.shape for p in params] != self._shapes or any(p.dtype != torch.float32 or p.device != self.device for p in params):
-                raise CodepsHipError("AdamW.step: a parameter has changed its shape, type or device since it was listed")
+            with torch.no_grad():
+                grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
+            ptrs, types, _, _ = bind().optimizer_lists(params, grads, self._table_addresses)
+        if moved:
+            if [p.shape for p in params] != self._shapes or any(p.dtype != torch.float32 or p.device != self.device or not _dense(p) for p in params):
+                raise CodepsHipError("AdamW.step: a parameter has changed its shape, type, layout or device since it was listed")
             if torch.cuda.is_current_stream_capturing():
                 raise CodepsHipError("AdamW.step: a parameter has moved since the last step: run one step before the capture")
             self._fill_items()
-        # addresses and types of the gradients: 0 = none (an empty tensor has no address, but a gradient)
-        ptrs = array.array("Q", map(torch.Tensor.data_ptr, some) if whole else [0 if g is None else g.data_ptr() for g in grads])
-        if 0 in self._numels:
-            ptrs = array.array("Q", [0 if g is None else p or 16 for p, g in zip(ptrs, grads)])
-        if not whole:
-            types = bytes([0 if g is None else F._TYPES[g.dtype] for g in grads])
         for c, g in zip(self._c_groups, self.param_groups):
             lr = g["lr"]
             if torch.is_tensor(lr):
@@ -191,9 +206,9 @@ class AdamW:
             else:
                 c.lr, c.lr_device = lr, None
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
-        F._launch(self.device, "codeps_adamw_step", lib().codeps_adamw_step, self._items.data_ptr(), len(params), self._chunk_items.data_ptr(), self._chunk0,
-                  ptrs.buffer_info()[0], types, self._c_numels, self._c_groups, len(self.param_groups), self.steps.data_ptr(), *map(F._at, self._states()),
-                  float(grad_scale), self.max_norm or 0.0, int(self.skip_nonfinite), F._at(self.grad_norm), self.seed, self.ema_alpha if apply_ema else -1.0,
+        _launch(self.device, "codeps_adamw_step", lib().codeps_adamw_step, self._items.data_ptr(), len(params), self._chunk_items.data_ptr(), self._chunk0,
+                  ptrs, types, self._c_numels, self._c_groups, len(self.param_groups), self.steps.data_ptr(), *map(_at, self._states()),
+                  float(grad_scale), self.max_norm or 0.0, int(self.skip_nonfinite), _at(self.grad_norm), self.seed, self.ema_alpha if apply_ema else -1.0,
                   self._ws.data_ptr(), self._ws.numel())
         torch.autograd.graph.increment_version(params)
         F.invalidate_weight_cache()
@@ -204,8 +219,8 @@ class AdamW:
             raise CodepsHipError("AdamW.moments_8bit: no tensor has 8-bit states")
         m = torch.empty(self._n8, dtype=torch.bfloat16, device=self.device)
         r = torch.empty_like(m)
-        F._launch(self.device, "codeps_adamw_moments_8bit", lib().codeps_adamw_moments_8bit, self._items.data_ptr(), len(self.params),
-                  self._chunk_items.data_ptr(), self._n_chunks, *map(F._at, self._states()[2:]), m.data_ptr(), r.data_ptr())
+        _launch(self.device, "codeps_adamw_moments_8bit", lib().codeps_adamw_moments_8bit, self._items.data_ptr(), len(self.params),
+                  self._chunk_items.data_ptr(), self._n_chunks, *map(_at, self._states()[2:]), m.data_ptr(), r.data_ptr())
         return m, r
 
     _STATES = ("steps", "exp_avg", "exp_avg_sq", "exp_avg_codes", "exp_avg_exponents", "root_codes", "root_exponents")

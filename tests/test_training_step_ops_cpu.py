@@ -13,8 +13,25 @@ from codeps_amd.optim import AdamW
 def test_cpu_tensors_are_refused():
     x = torch.zeros(3, 4)
     for call in (lambda: F.channel_norm(x), lambda: F.channel_norm_residual(x, x), lambda: AdamW([x]), lambda: F.grad_norm([x])):
+        with pytest.raises(CodepsHipError, match="GPU only"):
+            call()
+
+
+def test_wrong_kinds_of_arguments_are_refused():
+    x = torch.zeros(3, 4)
+    for call in (lambda: F.channel_norm(None), lambda: F.channel_norm([1.0]), lambda: F.channel_norm(x, 3), lambda: F.channel_norm(x, eps="small"),
+                 lambda: F.channel_norm(x, kind="batch"), lambda: F.channel_norm_residual(x, next_kind="x"), lambda: F.channel_norm_residual(x, gate_act="gelu"),
+                 lambda: F.channel_norm_residual(x, scale=None), lambda: F.grad_norm(None), lambda: F.grad_norm([1.0]), lambda: F.grad_norm([])):
         with pytest.raises(CodepsHipError):
             call()
+    native = _lib.bind()
+    for call in (lambda: native.channel_norm(x), lambda: native.grad_norm(), lambda: native.optimizer_lists([], []), lambda: native.init(1)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(CodepsHipError):
+        native.optimizer_lists([x], [x], b"")
+    with pytest.raises(CodepsHipError):
+        native.optimizer_lists([x], [], bytes(8))
 
 
 def _desc(**over):
