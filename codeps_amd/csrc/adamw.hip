@@ -140,13 +140,14 @@ template <int NT> __device__ __forceinline__ double block_sum64(double v, double
     return s;
 }
 
-// Each group of 256 threads walks its own contiguous range of chunks.  norm != NULL (one block of four groups): the norm itself, no partials and no second
-// launch -- up to 32 chunks, per call: 12 tensors of 3000 elements 13.1 -> 10.4 us, 32 of 4096 16.4 -> 13.7 us, one of 131072 11.3 -> 9.1 us.
-template <int NT> __global__ __launch_bounds__(NT) void grad_norm_kernel(NormTensors t, double* __restrict__ part, double scale, float* __restrict__ norm) {
+// Each group of GT threads walks its own contiguous range of chunks.  norm != NULL (one block): the norm itself, no partials and no second launch.  One block
+// (8 groups of 128) up to 32 chunks against two launches, per call: 12 tensors of 3000 elements 6.3 / 9.3 us, 32 of 4096 8.8 / 9.5 us, one of 131072
+// 7.9 / 9.4 us; 4 groups of 256 take 10.0, 16 of 64 8.6 us for the 32.
+template <int NT, int GT> __global__ __launch_bounds__(NT) void grad_norm_kernel(NormTensors t, double* __restrict__ part, double scale, float* __restrict__ norm) {
     __shared__ double red[NT / 64];
-    constexpr int GROUPS = NT / 256, K = NCHUNK / (256 * 4);
-    const int tid = threadIdx.x & 255;
-    const unsigned total = t.chunk0[t.count], group = blockIdx.x * GROUPS + (unsigned)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8), groups = gridDim.x * GROUPS;
+    constexpr int GROUPS = NT / GT, K = NCHUNK / (GT * 4);
+    const int tid = threadIdx.x & (GT - 1);
+    const unsigned total = t.chunk0[t.count], group = blockIdx.x * GROUPS + (unsigned)__builtin_amdgcn_readfirstlane((int)threadIdx.x / GT), groups = gridDim.x * GROUPS;
     const unsigned c0 = (unsigned)((unsigned long long)total * group / groups), c1 = (unsigned)((unsigned long long)total * (group + 1) / groups);
     int lo = 0, hi = t.count - 1;                                  // the last tensor that starts at or before chunk c0
     while (lo < hi) {
@@ -162,7 +163,7 @@ template <int NT> __global__ __launch_bounds__(NT) void grad_norm_kernel(NormTen
         const auto chunk = [&](auto tail) {
             float v[K][4];
 #pragma unroll
-            for (int k = 0; k < K; ++k) grad4<decltype(tail)::value>(g, type, i0 + k * 1024, n, v[k]);
+            for (int k = 0; k < K; ++k) grad4<decltype(tail)::value>(g, type, i0 + k * GT * 4, n, v[k]);
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -472,13 +473,13 @@ int norm_partials(const void* const* grads, const unsigned char* types, const lo
         t.chunk0[t.count] = (unsigned)chunks;
         if (chunks == 0) continue;
         if (norm && chunks <= ONE_BLOCK_CHUNKS && t.count == n) {
-            hipLaunchKernelGGL(grad_norm_kernel<1024>, dim3(1), dim3(1024), 0, st, t, part, scale, norm);
+            hipLaunchKernelGGL((grad_norm_kernel<1024, 128>), dim3(1), dim3(1024), 0, st, t, part, scale, norm);
             CODEPS_CHECK_LAUNCH("grad_norm_kernel");
             *finished = true;
             return 0;
         }
         const int blocks = (int)std::min<long long>(chunks, NORM_BLOCKS);
-        hipLaunchKernelGGL(grad_norm_kernel<THREADS>, dim3(blocks), dim3(THREADS), 0, st, t, part + parts, 1.0, (float*)nullptr);
+        hipLaunchKernelGGL((grad_norm_kernel<THREADS, THREADS>), dim3(blocks), dim3(THREADS), 0, st, t, part + parts, 1.0, (float*)nullptr);
         CODEPS_CHECK_LAUNCH("grad_norm_kernel");
         parts += blocks;
     }
