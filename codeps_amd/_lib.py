@@ -57,6 +57,15 @@ class AdamWGroup(Structure):
     _fields_ = [(n, c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [("lr_device", c_void_p)]
 
 
+class StepBlock(Structure):
+    """What stays the same from step to step (csrc/bind.cpp: StepBlock)."""
+    _fields_ = ([("items", c_void_p), ("n_items", ctypes.c_longlong), ("chunk_items", c_void_p), ("chunk0", c_void_p), ("numels", c_void_p),
+                 ("groups", c_void_p), ("n_groups", ctypes.c_longlong)] +
+                [(n, c_void_p) for n in ("steps", "exp_avg", "exp_avg_sq", "exp_avg_codes", "exp_avg_exponents", "root_codes", "root_exponents", "norm",
+                                         "workspace")] +
+                [("workspace_bytes", ctypes.c_ulonglong), ("seed", ctypes.c_ulonglong), ("addresses", c_void_p)])
+
+
 def build(jobs=8, verbose=False):
     """Compile every HIP source for gfx950 into the in-tree shared library (hipcc cross-compiles
     without a GPU)."""
@@ -299,7 +308,7 @@ def bind():
             raise CodepsHipError(f"codeps_amd/_bind.so cannot be loaded ({e}): build it with `make -C codeps_amd/csrc`") from e
         module.init(CodepsHipError, torch.OutOfMemoryError, *[ctypes.cast(getattr(handle, name), c_void_p).value for name in
                                       ("codeps_last_error", "codeps_channel_norm_fwd", "codeps_channel_norm_bwd_workspace_bytes", "codeps_channel_norm_bwd",
-                                       "codeps_grad_norm_workspace_bytes", "codeps_grad_norm")])
+                                       "codeps_grad_norm_workspace_bytes", "codeps_grad_norm", "codeps_adamw_step")])
         _bind = module
     return _bind
 

@@ -1,10 +1,10 @@
-// codeps_amd/_bind.so: the Python side of the channel norms, AdamW's lists and the gradient norm, in C++ on torch's own API (tensors, autograd nodes).
+// codeps_amd/_bind.so: the Python side of the channel norms, AdamW's step and the gradient norm, in C++ on torch's own API (tensors, autograd nodes).
 // The arithmetic is in libcodeps_hip.so behind its C ABI (include/codeps_hip.h), whose entry points this module is handed as addresses, so that both follow
 // the one library that the package has loaded.
 //
 // Why not ctypes and torch.autograd.Function as elsewhere: these calls are short.  A backward pass written in Python runs on autograd's worker thread and
 // has to wait for the interpreter lock there; a list of 160 gradients costs 0.2 us per tensor in Python.  Per call, Python / this module: one-row norm
-// 9.4 / 6.1 us, small norm with its gradients 103 / 69 us, gradient norm of 160 small tensors 37 / 12 us, AdamW's step over them 54 / 20 us.
+// 9.4 / 6.1 us, small norm with its gradients 103 / 69 us, gradient norm of 160 small tensors 37 / 12 us, AdamW's step over them 54 / 13 us.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -36,6 +36,7 @@ struct {
     decltype(&codeps_channel_norm_bwd) norm_bwd;
     decltype(&codeps_grad_norm_workspace_bytes) grad_norm_bytes;
     decltype(&codeps_grad_norm) grad_norm;
+    decltype(&codeps_adamw_step) adamw_step;
 } api;
 PyObject *error_class = nullptr, *memory_error = nullptr;              // CodepsHipError, torch.OutOfMemoryError
 
@@ -416,42 +417,75 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
     });
 }
 
-// optimizer_lists(params, grads, addresses) -> (gradient addresses, their types, moved, mixed): both as bytes for the C ABI; 0 = no gradient.
-// moved: a parameter is not where `addresses` (bytes of 64-bit numbers) says; mixed: a gradient lies in another order than its parameter.
-PyObject* py_optimizer_lists(PyObject*, PyObject* const* a, Py_ssize_t na) {
-    if (!count(na, 3)) return nullptr;
+// What stays the same from step to step (codeps_amd.optim.AdamW fills it once, as a ctypes structure with these fields)
+struct StepBlock {
+    const void* items;
+    long long n_items;
+    const int* chunk_items;
+    const long long *chunk0, *numels;
+    const codeps_adamw_group* groups;
+    long long n_groups;
+    long long* steps;
+    float *exp_avg, *exp_avg_sq;
+    unsigned char *exp_avg_codes, *exp_avg_exponents, *root_codes, *root_exponents;
+    float* norm;
+    void* workspace;
+    unsigned long long workspace_bytes, seed;
+    const unsigned long long* addresses;                              // where the parameters and the tensors beside them were when the items were filled
+};
+
+// adamw_step(params, beside, grads, address of the StepBlock, grad_scale, max_norm, skip_nonfinite, ema_alpha) -> 0 when the step is launched; without a
+// launch 1: a parameter or a tensor beside it (EMA, copy) has moved, 2: a gradient lies in another order than its parameter, 3: both
+PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    if (!count(na, 8)) return nullptr;
     return guarded([&]() -> PyObject* {
         const char* what = "AdamW.step";
-        const Sequence params(a[0]), grads(a[1]);
+        const Sequence params(a[0]), beside(a[1]), grads(a[2]);
+        const StepBlock* block = PyLong_Check(a[3]) ? (const StepBlock*)PyLong_AsVoidPtr(a[3]) : nullptr;
         const Py_ssize_t n = params.size();
+        if (!block) refuse(what, ": no step block");
+        if (block->n_items != n) refuse(what, ": ", n, " parameters, ", block->n_items, " were listed");
         if (grads.size() != n) refuse(what, ": one gradient (or None) per parameter (", n, "), got ", grads.size());
-        const uint64_t* was = (const uint64_t*)PyBytes_AsString(a[2]);
-        if (!was || PyBytes_Size(a[2]) != n * 8) refuse(what, ": the table of addresses does not fit");
-        std::vector<uint64_t> ptrs(n);
+        const double grad_scale = number(a[4]), max_norm = number(a[5]), ema_alpha = number(a[7]);
+        const int skip = a[6] == Py_True;
+        std::vector<const void*> ptrs(n);
         std::vector<unsigned char> types(n);
         bool moved = false, mixed = false;
         for (Py_ssize_t i = 0; i < n; ++i) {
             if (!THPVariable_Check(params[i])) refuse(what, ": parameters are tensors, got ", Py_TYPE(params[i])->tp_name);
             const Tensor& p = THPVariable_Unpack(params[i]);
-            moved = moved || (uint64_t)(uintptr_t)p.data_ptr() != was[i];
+            moved = moved || (unsigned long long)(uintptr_t)p.data_ptr() != block->addresses[i] || p.numel() != block->numels[i];
             if (grads[i] == Py_None) continue;
             if (!THPVariable_Check(grads[i])) refuse(what, ": gradients are tensors or None, got ", Py_TYPE(grads[i])->tp_name);
             const Tensor& g = THPVariable_Unpack(grads[i]);
             check_gradient(g, p.device(), what);
             if (g.sizes() != p.sizes()) refuse(what, ": gradient ", i, " is ", g.sizes(), ", its parameter ", p.sizes());
             mixed = mixed || !dense(p) || !(g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous()));
-            ptrs[i] = g.numel() ? (uint64_t)(uintptr_t)g.data_ptr() : 16;              // (an empty tensor has no address, but a gradient)
+            ptrs[i] = g.numel() ? g.data_ptr() : (const void*)16;                      // (an empty tensor has no address, but a gradient)
             types[i] = (unsigned char)type_of(g);
         }
-        return Py_BuildValue("(y#y#NN)", (const char*)ptrs.data(), (Py_ssize_t)(n * 8), (const char*)types.data(), n, PyBool_FromLong(moved), PyBool_FromLong(mixed));
+        for (Py_ssize_t i = 0; i < beside.size() && !moved; ++i)
+            moved = !THPVariable_Check(beside[i]) || (unsigned long long)(uintptr_t)THPVariable_Unpack(beside[i]).data_ptr() != block->addresses[n + i];
+        if (moved || mixed) return PyLong_FromLong((moved ? 1 : 0) | (mixed ? 2 : 0));
+        const Tensor& first = THPVariable_Unpack(params[0]);
+        c10::DeviceGuard guard(first.device());
+        check(api.adamw_step(block->items, (int)n, block->chunk_items, block->chunk0, ptrs.data(), types.data(), block->numels, block->groups, (int)block->n_groups,
+                             block->steps, block->exp_avg, block->exp_avg_sq, block->exp_avg_codes, block->exp_avg_exponents, block->root_codes,
+                             block->root_exponents, grad_scale, max_norm, skip, block->norm, block->seed, ema_alpha, block->workspace,
+                             (size_t)block->workspace_bytes, stream_of(first)), "codeps_adamw_step");
+        for (Py_ssize_t i = 0; i < n; ++i) {                          // saved tensors of a graph that is still to run backward must notice
+            const Tensor& p = THPVariable_Unpack(params[i]);
+            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        }
+        return PyLong_FromLong(0);
     });
 }
 
 // init(CodepsHipError, torch.OutOfMemoryError, addresses of the C entries in the order of `api`)
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t na) {
-    if (!count(na, 8)) return nullptr;
-    void* p[6];
-    for (int i = 0; i < 6; ++i) {
+    if (!count(na, 9)) return nullptr;
+    void* p[7];
+    for (int i = 0; i < 7; ++i) {
         p[i] = PyLong_AsVoidPtr(a[2 + i]);
         if (!p[i]) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
@@ -468,6 +502,7 @@ PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t na) {
     api.norm_bwd = (decltype(api.norm_bwd))p[3];
     api.grad_norm_bytes = (decltype(api.grad_norm_bytes))p[4];
     api.grad_norm = (decltype(api.grad_norm))p[5];
+    api.adamw_step = (decltype(api.adamw_step))p[6];
     Py_RETURN_NONE;
 }
 
@@ -475,7 +510,7 @@ PyMethodDef methods[] = {{"init", (PyCFunction)(void*)py_init, METH_FASTCALL, nu
                          {"channel_norm", (PyCFunction)(void*)py_channel_norm, METH_FASTCALL, nullptr},
                          {"channel_norm_residual", (PyCFunction)(void*)py_channel_norm_residual, METH_FASTCALL, nullptr},
                          {"grad_norm", (PyCFunction)(void*)py_grad_norm, METH_FASTCALL, nullptr},
-                         {"optimizer_lists", (PyCFunction)(void*)py_optimizer_lists, METH_FASTCALL, nullptr},
+                         {"adamw_step", (PyCFunction)(void*)py_adamw_step, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Python side of the training-step operators", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -4,32 +4,20 @@
     loss.backward(); opt.step(); opt.zero_grad()
 
 Next to functional.adam_ema_step (Adam on flat fp32 buffers): decoupled weight decay, parameters that lie anywhere, gradients of any of the three float
-types, global-norm clipping inside the step, 8-bit states.  A step is two launches for all tensors (four with clipping), whatever their number up to 320.
+types, global-norm clipping inside the step, 8-bit states.  A step is two launches for up to 320 tensors,
+with clipping three for up to 160.
 Step counts, the clipping factor and the random bits of the 8-bit rounding live on the device: a captured step() replays as the next step.
 """
-import array
 import ctypes
 
 import torch
 
 from . import functional as F
-from ._lib import AdamWGroup, CodepsHipError, bind, check, lib, ptr, require_cuda
+from ._lib import AdamWGroup, CodepsHipError, StepBlock, bind, check, lib, ptr, require_cuda, stream_ptr
 
 BLOCK = 256                     # elements of one tensor that share an exponent byte
 CHUNK = 2048                    # elements of one tensor that a work group updates
 MAX_GROUPS = 16
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream          # (device index) -> hipStream_t; torch.cuda.current_stream builds an object (4 us)
-
-
-def _launch(device, what, call, *args):
-    """check(call(*args, stream)) on the current stream of `device`, which need not be the current device."""
-    if device.index == torch._C._cuda_getDevice():
-        check(call(*args, _raw_stream(device.index)), what)
-    else:
-        with torch.cuda.device(device):
-            check(call(*args, _raw_stream(device.index)), what)
 
 
 def _at(t):
@@ -108,6 +96,8 @@ class AdamW:
         self.ema_alpha, self.max_norm, self.skip_nonfinite, self.seed = float(ema_alpha), max_norm, bool(skip_nonfinite), int(seed)
         if max_norm is not None and not max_norm > 0:
             raise CodepsHipError(f"AdamW: max_norm = {max_norm}")
+        if not 0.0 <= self.ema_alpha <= 1.0:
+            raise CodepsHipError(f"AdamW: ema_alpha = {ema_alpha}")
         # ---- states: the 32-bit tensors packed, the 8-bit ones in whole blocks
         self._numels = [p.numel() for p in self.params]
         self._offsets, self._packed, chunk0, n32, n8, packed = [], [], [0], 0, 0, 0
@@ -130,7 +120,7 @@ class AdamW:
         self._n8 = packed
         want_norm = max_norm is not None or self.skip_nonfinite
         self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev) if want_norm else None
-        # ---- launch tables
+        # ---- launch tables (csrc/bind.cpp: the step's constant part is handed over as one structure)
         self._chunk0 = (ctypes.c_longlong * (n + 1))(*chunk0)
         self._n_chunks = chunk0[-1]
         counts = torch.tensor([b - a for a, b in zip(chunk0, chunk0[1:])])
@@ -139,8 +129,13 @@ class AdamW:
         self._c_groups = (AdamWGroup * len(self.param_groups))()
         self._shapes = [p.shape for p in self.params]
         self._items = torch.zeros(n * lib().codeps_adamw_item_bytes(), dtype=torch.uint8, device=dev)
+        self._by = [t for t in self._ema + self._copies if t is not None]
+        self._c_addresses = (ctypes.c_ulonglong * (n + len(self._by)))()
         self._fill_items()
         self._ws = torch.empty(lib().codeps_adamw_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        self._c_step = StepBlock(self._items.data_ptr(), n, self._chunk_items.data_ptr(), ctypes.addressof(self._chunk0), ctypes.addressof(self._c_numels),
+                                 ctypes.addressof(self._c_groups), len(self.param_groups), self.steps.data_ptr(), *map(_at, self._states()), _at(self.grad_norm),
+                                 self._ws.data_ptr(), self._ws.numel(), self.seed, ctypes.addressof(self._c_addresses))
 
     def _beside(self, tensors, dtypes, what):
         """ema / copies: one tensor (or None) per parameter, with its shape and layout."""
@@ -152,11 +147,11 @@ class AdamW:
                 raise CodepsHipError(f"AdamW: {what}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with a parameter of {tuple(p.shape)}")
         return tensors
 
-    def _addresses(self):
-        return array.array("Q", [t.data_ptr() for t in self.params]).tobytes()
-
     def _fill_items(self):
         """(Re)writes the device table in place: a captured step reads the same table."""
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.params + self._by if t.numel())
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise CodepsHipError("AdamW: parameters, EMA tensors or copies share memory")
         size = lib().codeps_adamw_item_bytes()
         host = ctypes.create_string_buffer(size * len(self.params))
         base = ctypes.addressof(host)
@@ -166,7 +161,7 @@ class AdamW:
             if k < 0:
                 raise CodepsHipError("codeps_adamw_item_fill: " + lib().codeps_last_error().decode())
         self._items.copy_(torch.frombuffer(bytearray(host.raw), dtype=torch.uint8))
-        self._table_addresses = self._addresses()
+        self._c_addresses[:] = [t.data_ptr() for t in self.params + self._by]
 
     def _states(self):
         return self.exp_avg, self.exp_avg_sq, self.exp_avg_codes, self.exp_avg_exponents, self.root_codes, self.root_exponents
@@ -183,20 +178,7 @@ class AdamW:
         The others keep value, states and step count.  grad_scale multiplies the gradients (1 / world size after a summing all-reduce); apply_ema False
         leaves the EMA tensors alone."""
         params = self.params
-        grads = [p.grad for p in params] if grads is None else grads
-        ptrs, types, moved, mixed = bind().optimizer_lists(params, grads, self._table_addresses)
-        if mixed:
-            if any(p.numel() != k or not _dense(p) for p, k in zip(params, self._numels)):
-                raise CodepsHipError("AdamW.step: a parameter has changed its shape or layout since it was listed")
-            with torch.no_grad():
-                grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
-            ptrs, types, _, _ = bind().optimizer_lists(params, grads, self._table_addresses)
-        if moved:
-            if [p.shape for p in params] != self._shapes or any(p.dtype != torch.float32 or p.device != self.device or not _dense(p) for p in params):
-                raise CodepsHipError("AdamW.step: a parameter has changed its shape, type, layout or device since it was listed")
-            if torch.cuda.is_current_stream_capturing():
-                raise CodepsHipError("AdamW.step: a parameter has moved since the last step: run one step before the capture")
-            self._fill_items()
+        grads = [p.grad for p in params] if grads is None else list(grads)
         for c, g in zip(self._c_groups, self.param_groups):
             lr = g["lr"]
             if torch.is_tensor(lr):
@@ -206,11 +188,23 @@ class AdamW:
             else:
                 c.lr, c.lr_device = lr, None
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
-        _launch(self.device, "codeps_adamw_step", lib().codeps_adamw_step, self._items.data_ptr(), len(params), self._chunk_items.data_ptr(), self._chunk0,
-                  ptrs, types, self._c_numels, self._c_groups, len(self.param_groups), self.steps.data_ptr(), *map(_at, self._states()),
-                  float(grad_scale), self.max_norm or 0.0, int(self.skip_nonfinite), _at(self.grad_norm), self.seed, self.ema_alpha if apply_ema else -1.0,
-                  self._ws.data_ptr(), self._ws.numel())
-        torch.autograd.graph.increment_version(params)
+        rest = (ctypes.addressof(self._c_step), grad_scale, self.max_norm or 0.0, self.skip_nonfinite, self.ema_alpha if apply_ema else -1.0)
+        state = bind().adamw_step(params, self._by, grads, *rest)
+        if state & 1:
+            if [p.shape for p in params] != self._shapes or any(p.dtype != torch.float32 or p.device != self.device or not _dense(p) for p in params):
+                raise CodepsHipError("AdamW.step: a parameter has changed its shape, type, layout or device since it was listed")
+            if torch.cuda.is_current_stream_capturing():
+                raise CodepsHipError("AdamW.step: a parameter (or a tensor beside it) has moved since the last step: run one step before the capture")
+            self._beside(self._ema, (torch.float32,), "ema")
+            self._beside(self._copies, (torch.bfloat16, torch.float16), "copies")
+            self._fill_items()
+        if state & 2:
+            if not all(map(_dense, params)):
+                raise CodepsHipError("AdamW.step: a parameter has changed its layout since it was listed")
+            with torch.no_grad():
+                grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
+        if state and bind().adamw_step(params, self._by, grads, *rest):
+            raise CodepsHipError("AdamW.step: a parameter or gradient changes under the step")
         F.invalidate_weight_cache()
 
     def moments_8bit(self):
@@ -219,9 +213,13 @@ class AdamW:
             raise CodepsHipError("AdamW.moments_8bit: no tensor has 8-bit states")
         m = torch.empty(self._n8, dtype=torch.bfloat16, device=self.device)
         r = torch.empty_like(m)
-        _launch(self.device, "codeps_adamw_moments_8bit", lib().codeps_adamw_moments_8bit, self._items.data_ptr(), len(self.params),
-                  self._chunk_items.data_ptr(), self._n_chunks, *map(_at, self._states()[2:]), m.data_ptr(), r.data_ptr())
+        with torch.cuda.device(self.device):
+            check(lib().codeps_adamw_moments_8bit(ptr(self._items), len(self.params), ptr(self._chunk_items), self._n_chunks, *map(ptr, self._states()[2:]), ptr(m),
+                                                  ptr(r), stream_ptr()), "codeps_adamw_moments_8bit")
         return m, r
+
+    def __reduce__(self):
+        raise CodepsHipError("AdamW holds device addresses: pass on its state_dict()")
 
     _STATES = ("steps", "exp_avg", "exp_avg_sq", "exp_avg_codes", "exp_avg_exponents", "root_codes", "root_exponents")
 

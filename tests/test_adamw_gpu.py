@@ -4,6 +4,7 @@ Tolerances (fixed before the first run).  32-bit states: a moment is two product
 step, and errors of earlier steps only decay: 8 * 2^-24 * (|b1 m| + |(1 - b1) g'|) per step, twice that for v (g' is squared).  The parameter adds its own
 rounding and lr * 32 * 2^-24 of the ratio, whose error is that of m, sqrt(v), a reciprocal and two scalars; m may cancel, so its error counts relative to
 its terms.  8-bit states: codes and exponents are EQUAL to those of the 64-bit formula (the kernel decides in 64 bits where fp32 could be wrong)."""
+import copy
 import math
 
 import numpy as np
@@ -463,3 +464,42 @@ def test_refusals():
         AdamW([p], lr=torch.zeros(2, device=DEV)).step([p])
     with pytest.raises(CodepsHipError):
         AdamW([p]).moments_8bit()
+
+
+def test_tensors_that_share_memory_are_refused():
+    """Two work groups would update the same elements."""
+    p = torch.zeros(100, device=DEV)
+    half = torch.zeros(64, dtype=BF16, device=DEV)
+    for bad in (lambda: AdamW([p, p[50:]]), lambda: AdamW([p[:10], p], ema=[torch.zeros(10, device=DEV), None]), lambda: AdamW([p], ema=[p]),
+                lambda: AdamW([p[:50], p[50:]], ema=[torch.zeros(50, device=DEV), p[:50]]), lambda: AdamW([p[:32], p[32:64]], copies=[half[:32], half[16:48]]),
+                lambda: AdamW([p], ema_alpha=-0.1), lambda: AdamW([p], ema_alpha=float("nan")), lambda: copy.deepcopy(AdamW([p]))):
+        with pytest.raises(CodepsHipError):
+            bad()
+    AdamW([p[:50], p[50:]], copies=[half[:0].new_zeros(50), None])                        # neighbours do not
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_that_move_between_steps(bits):
+    """.data = of parameters, EMA tensors and copies: the next step writes where they are, and nothing where they were."""
+    p, e, c = tensors([5000], 1)[0], torch.zeros(5000, device=DEV), torch.zeros(5000, dtype=BF16, device=DEV)
+    q, f = p.clone(), e.clone()
+    a, b = AdamW([p], lr=1e-2, state_bits=bits, ema=[e], copies=[c]), AdamW([q], lr=1e-2, state_bits=bits, ema=[f])
+    for k in range(6):
+        if k in (1, 4):
+            p.data = p.data.clone()
+        old = {2: e, 3: c}.get(k)
+        if old is not None:
+            was, before = old.data, old.data.clone()
+            old.data = old.data.clone()
+        g = gradients([q], 30 + k)
+        a.step(g)
+        b.step(g)
+        assert torch.equal(p, q) and torch.equal(e, f) and torch.equal(c, p.to(BF16)), k
+        assert old is None or torch.equal(was, before), k
+    e.data = e.data.half()
+    with pytest.raises(CodepsHipError):
+        a.step(g)
+    with pytest.raises(CodepsHipError):
+        a.step(iter(g + g))
+    b.step(iter(g))                                                  # (any iterable serves)
+    assert b.steps.tolist() == [7]

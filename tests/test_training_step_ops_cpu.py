@@ -25,13 +25,16 @@ def test_wrong_kinds_of_arguments_are_refused():
         with pytest.raises(CodepsHipError):
             call()
     native = _lib.bind()
-    for call in (lambda: native.channel_norm(x), lambda: native.grad_norm(), lambda: native.optimizer_lists([], []), lambda: native.init(1)):
+    for call in (lambda: native.channel_norm(x), lambda: native.grad_norm(), lambda: native.adamw_step([], []), lambda: native.init(1)):
         with pytest.raises(TypeError):
             call()
-    with pytest.raises(CodepsHipError):
-        native.optimizer_lists([x], [x], b"")
-    with pytest.raises(CodepsHipError):
-        native.optimizer_lists([x], [], bytes(8))
+    numels, places = (ctypes.c_longlong * 1)(12), (ctypes.c_ulonglong * 1)(x.data_ptr())
+    block = _lib.StepBlock(n_items=1, numels=ctypes.addressof(numels), addresses=ctypes.addressof(places))
+    at = ctypes.addressof(block)
+    for args in (([x], [], [x], 0), ([x], [], [x], None), ([x], [], [], at), ([x, x], [], [x, x], at), ([1], [], [x], at), ([x], [], [2], at), ([x], None, [x], at),
+                 ([x], [], [x], at)):
+        with pytest.raises(CodepsHipError):
+            native.adamw_step(*args, 1.0, 0.0, False, 0.9)
 
 
 def _desc(**over):
@@ -112,4 +115,5 @@ def test_adamw_entries_check_their_arguments():
 
 def test_struct_layouts():
     assert ctypes.sizeof(_lib.ChannelNormDesc) == 112 and _lib.ChannelNormDesc.channels.offset == 48 and _lib.ChannelNormDesc.scale.offset == 96
+    assert ctypes.sizeof(_lib.StepBlock) == 19 * 8
     assert ctypes.sizeof(_lib.AdamWGroup) == 48 and _lib.AdamWGroup.lr_device.offset == 40
