@@ -10,7 +10,9 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -162,12 +164,16 @@ struct ChannelNormBackward : public torch::autograd::Node {
         if (res) out[1] = d.next_kind ? at::empty(x_sizes, res_options) : given;
         if (task_should_compute_output(2)) out[2] = d.rows ? at::empty(gate_sizes, gate_options) : at::zeros(gate_sizes, gate_options);
         void* vec[4] = {};
+        Tensor twice[4];                                              // one parameter as two of the vectors: the second gradient is added behind the pass
         int acc = 0;
         for (int i = 0; i < (d.next_kind ? 4 : 2); ++i) {
             if (!task_should_compute_output(3 + i)) continue;
             if (sinks[i].defined()) {
                 vec[i] = sinks[i].data_ptr();
-                acc |= 1 << i;
+                for (int j = 0; j < i; ++j)
+                    if (vec[j] == vec[i]) twice[i] = at::empty({d.channels}, sinks[i].options());
+                if (twice[i].defined()) vec[i] = twice[i].data_ptr();
+                else acc |= 1 << i;
             } else {
                 out[3 + i] = at::empty({d.channels}, vec_options[i]);
                 vec[i] = out[3 + i].data_ptr();
@@ -180,9 +186,26 @@ struct ChannelNormBackward : public torch::autograd::Node {
         check(api.norm_bwd(&d, at_(xs), at_(rs), at_(gs), at_(ws), at_(bs), at_(nws), (const float*)at_(st), at_(dy), at_(dh), at_(out[0]),
                            res && d.next_kind ? at_(out[1]) : nullptr, at_(out[2]), vec[0], vec[1], vec[2], vec[3], acc, work.data_ptr(), bytes, stream_of(xs)),
               "codeps_channel_norm_bwd");
+        for (int i = 0; i < 4; ++i)
+            if (twice[i].defined()) sinks[i].add_(twice[i].view(sinks[i].sizes()));
         return out;
     }
 };
+
+// A leaf's accumulation node runs on the stream that was current when its oldest living graph was built.  Where that is the default stream and the current
+// one is captured, the backward pass would put work on a stream that cannot be captured, in the middle of a capture: refused while nothing has happened yet.
+void check_capture(const Tensor* const (&in)[7]) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : in) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        if (stream && stream->id() == c10::hip::getDefaultHIPStream(t->device().index()).id())
+            refuse("channel norm under graph capture: a graph that was built eagerly on the default stream still refers to a leaf of shape ", t->sizes(),
+                   "; drop it before the capture, or build it on another stream");
+    }
+}
 
 // y[, h] or h, with a node behind them where a gradient is wanted; sinks: 4 tensors, undefined where there is none
 void apply(Norm& n, const Tensor (&sinks)[4]) {
@@ -190,6 +213,7 @@ void apply(Norm& n, const Tensor (&sinks)[4]) {
     bool grad = false;
     if (at::GradMode::is_enabled())
         for (const Tensor* t : in) grad = grad || (t->defined() && t->requires_grad());
+    if (grad) check_capture(in);
     {
         at::NoGradGuard off;
         forward(n, grad);
@@ -255,6 +279,8 @@ template <typename F> PyObject* guarded(F&& f) {
         return f();
     } catch (const Refused& e) {
         PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
+    } catch (python_error& e) {                                       // from a hook on saved tensors (re-computation ends its pass with one)
+        e.restore();
     } catch (const c10::OutOfMemoryError& e) {
         PyErr_SetString(memory_error ? memory_error : PyExc_MemoryError, e.what_without_backtrace());
     } catch (const c10::Error& e) {

@@ -387,6 +387,10 @@ extern "C" int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const 
     CODEPS_REQUIRE((!(accumulate & (CODEPS_ACC_WEIGHT | CODEPS_ACC_BIAS)) || d->weight_type == CODEPS_F32) &&
                    (!(accumulate & (CODEPS_ACC_NEXT_WEIGHT | CODEPS_ACC_NEXT_BIAS)) || d->next_weight_type == CODEPS_F32), CODEPS_ERR_ARG,
                    "channel_norm_bwd: gradients are accumulated in fp32 only");
+    const void* const outs[] = {dx, dresidual, dgate, dweight, dbias, dnext_weight, dnext_bias};
+    for (int i = 0; i < 7; ++i)
+        for (int j = 0; j < i; ++j)
+            CODEPS_REQUIRE(!outs[i] || outs[i] != outs[j], CODEPS_ERR_ARG, "channel_norm_bwd: two gradients have one address");
     if (d->rows > 0) {
         CODEPS_REQUIRE(x && stats && (!d->gate_mode || gate) && (d->full ? (dy || d->next_kind) : dh != nullptr) && (!d->next_kind || dh), CODEPS_ERR_ARG,
                        "channel_norm_bwd: null pointer");

@@ -2354,7 +2354,7 @@ def _sinks(*vectors):
     """The vectors' flat-gradient views, None where there is none (register_grad_sink), or None when nothing is registered."""
     if not _grad_sink:
         return None
-    return tuple(grad_sink(v) if v is not None and v.requires_grad else None for v in vectors)
+    return tuple(grad_sink(v) if getattr(v, "requires_grad", False) else None for v in vectors)
 
 
 def channel_norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):

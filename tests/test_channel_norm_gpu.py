@@ -338,6 +338,35 @@ def test_two_captured_graphs_replay_side_by_side():
                 assert torch.equal(o[k], w[k]), (seed, k)
 
 
+def test_capture_while_an_eager_graph_of_the_same_leaf_lives_is_refused():
+    """Its gradient would be accumulated on the default stream in the middle of the capture.  Without that graph the capture works."""
+    x, w, dh = torch.randn(9, 40, device=DEV), torch.nn.Parameter(torch.randn(40, device=DEV)), torch.randn(9, 40, device=DEV)
+    live = F.channel_norm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = x + 1.0
+        for call in (lambda: F.channel_norm(x, w), lambda: F.channel_norm_residual(x, next_kind="rms", next_weight=w)):
+            with pytest.raises(CodepsHipError, match="drop it before the capture"):
+                call()
+        with torch.no_grad():
+            F.channel_norm(x, w)                                     # (nothing to accumulate)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept, x + 1.0)
+    del live
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        F.channel_norm(x, w).backward(dh)
+    mine = w.grad
+    for seed in (1, 2, 3):
+        x.copy_(torch.randn(9, 40, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = w.detach().clone().requires_grad_(True)
+        F.channel_norm(x, fresh).backward(dh)
+        assert torch.equal(mine, fresh.grad), seed
+
+
 def test_gradients_go_straight_into_registered_sinks():
     c = case(50, (40,))
     t = make(c, 6)
@@ -352,6 +381,47 @@ def test_gradients_go_straight_into_registered_sinks():
     assert all(p.grad is None for p in params) and torch.equal(x.grad, want["dx"])
     for i, k in enumerate(VECTORS):
         assert torch.equal(flat[50 * i:50 * i + 50], torch.arange(50 * i, 50 * i + 50, dtype=F32, device=DEV) + want["d" + k]), k
+
+
+def test_one_parameter_as_both_norms_vectors():
+    """Shared by the two norms of a block's end, with and without a sink: the gradients add up (two roundings of 2^-24 more: the sum, and the sink's)."""
+    c = case(50, (400,))
+    t = make(c, 6)
+    t["next_weight"], t["next_bias"] = t["weight"], t["bias"]
+    apart = run(c, t)
+    x = t["x"].detach()
+    for sink in (False, True):
+        w, b = (torch.nn.Parameter(t[k].clone()) for k in ("weight", "bias"))
+        flat = torch.zeros(100, device=DEV)
+        if sink:
+            F.register_grad_sink(w, flat[:50])
+            F.register_grad_sink(b, flat[50:])
+        for n in (1, 2):
+            y, h = F.channel_norm_residual(x, t["residual"], w, b, scale=0.5, next_kind="layer", next_weight=w, next_bias=b)
+            torch.autograd.backward([y, h], [t["dy"], t["dh"]])
+            got = (flat[:50], flat[50:]) if sink else (w.grad, b.grad)
+            for g, k in zip(got, ("weight", "bias")):
+                parts = apart["d" + k].double(), apart["dnext_" + k].double()
+                bar = 4 * n * U * (parts[0].abs() + parts[1].abs())
+                assert ((g.double() - n * (parts[0] + parts[1])).abs() <= bar).all(), (sink, n, k)
+
+
+def test_block_end_of_one_tensor_and_under_checkpointing():
+    """x as its own residual: both gradients reach it.  Re-computation (torch.utils.checkpoint) gives the same bits."""
+    from torch.utils.checkpoint import checkpoint
+    c = case(48, (70,), gate="channel", act="silu")
+    t = make(c, 3)
+    leaves = [t[k].detach().clone().requires_grad_(True) for k in ("x", "gate") + VECTORS]
+
+    def block(x, gate, w, b, nw, nb):
+        return F.channel_norm_residual(x, x, w, b, scale=0.5, gate=gate, gate_act="silu", next_kind="layer", next_weight=nw, next_bias=nb)
+    plain = torch.autograd.grad(block(*leaves), leaves, [t["dy"], t["dh"]])
+    again = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, [t["dy"], t["dh"]])
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    x, other = (leaves[0].detach().clone().requires_grad_(True) for _ in range(2))
+    y, h = F.channel_norm_residual(x, other, *leaves[2:4], scale=0.5, gate=leaves[1], gate_act="silu", next_kind="layer", next_weight=leaves[4], next_bias=leaves[5])
+    parts = torch.autograd.grad([y, h], [x, other], [t["dy"], t["dh"]])
+    assert torch.equal(plain[0], parts[0] + parts[1])
 
 
 def test_rows_far_apart():

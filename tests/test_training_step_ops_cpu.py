@@ -73,7 +73,10 @@ def test_channel_norm_null_pointers_and_workspaces_are_refused():
     assert lib.codeps_channel_norm_bwd(ctypes.byref(d), *args, 16, fake, need, None) == -1
     assert lib.codeps_channel_norm_bwd(ctypes.byref(_desc(weight_type=1)), *args, 1, fake, need, None) == -1
     assert lib.codeps_channel_norm_bwd(ctypes.byref(_desc(dy_pitch=7)), *args, 0, fake, need, None) == -1
-    no_dy = list(args)
+    apart = [fake] * 9 + [64 * (i + 2) for i in range(7)]
+    for i in range(10, 16):                                          # two gradients at one address
+        assert lib.codeps_channel_norm_bwd(ctypes.byref(d), *apart[:i], apart[i - 1], *apart[i + 1:], 0, fake, need, None) == -1
+    no_dy = list(apart)
     no_dy[7] = None                                                  # neither dy nor a next norm
     assert lib.codeps_channel_norm_bwd(ctypes.byref(d), *no_dy, 0, fake, need, None) == -1
     assert lib.codeps_channel_norm_fwd(ctypes.byref(_desc(rows=0)), *[None] * 11) == 0
