@@ -75,44 +75,55 @@ template <int V, typename T> __device__ __forceinline__ void store_full(T* p, co
 template <typename T> __device__ __forceinline__ const T* at(const T* row, int c) { return (const T*)((const char*)row + (unsigned)c * (unsigned)sizeof(T)); }
 template <typename T> __device__ __forceinline__ T* at(T* row, int c) { return (T*)((char*)row + (unsigned)c * (unsigned)sizeof(T)); }
 
-// V channels from c0 on of the row that lies `off` elements behind `row`.  Whole pieces (TAIL false): a lane behind the row's end reads the row's first piece,
-// which its caller leaves out of every sum and every store.  TAIL: the piece that crosses the end is read from the row's last V elements and shifted;
-// elements past the end are 0.
-template <int V, bool TAIL, typename T> __device__ __forceinline__ void load_piece(const T* row, int off, int c0, int C, float* o) {
-    if constexpr (!TAIL) {
-        load_full<V>(at(row, off + (c0 < C ? c0 : 0)), o);
-    } else if (C >= V) {
-        // the shift works on the loaded words, two 16-bit elements at a time
-        constexpr int PER = sizeof(T) == 4 ? 1 : 2, W = V / PER;              // elements per word, words
-        const int first = min(c0, C - V), sh = c0 - first;
-        const T* p = at(row, off + first);
-        unsigned r[W];
+// V channels from c0 on of the row that lies `off` elements behind `row`, as they lie in memory.  Whole pieces (TAIL false): a lane behind the row's end reads
+// the row's first piece, which its caller leaves out of every sum and every store.  TAIL: the piece that crosses the end is read from the row's last V
+// elements and shifted by widen_piece; elements past the end are 0.
+template <int V, typename T> struct Raw { unsigned w[V * sizeof(T) / 4]; };
+template <int V, bool TAIL, typename T> __device__ __forceinline__ Raw<V, T> raw_piece(const T* row, int off, int c0, int C) {
+    constexpr int PER = 4 / sizeof(T), W = V / PER;                           // elements per word, words
+    Raw<V, T> r;
+    if (TAIL && C < V) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) r.w[e] = 0;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (c0 + e < C) r.w[e / PER] |= (PER == 1 ? ((const unsigned*)(const void*)at(row, off + c0))[e]
+                                                      : (unsigned)((const unsigned short*)(const void*)at(row, off + c0))[e] << (16 * (e % PER)));
+    } else {
+        const char* p = reinterpret_cast<const char*>(at(row, off + (TAIL ? min(c0, C - V) : c0 < C ? c0 : 0)));
 #pragma unroll
         for (int k = 0; k < W / 4; ++k) {
-            const u32x4u q = *reinterpret_cast<const u32x4u*>(reinterpret_cast<const char*>(p) + 16 * k);
+            const u32x4u q = *reinterpret_cast<const u32x4u*>(p + 16 * k);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[4 * k + e] = q[e];
+            for (int e = 0; e < 4; ++e) r.w[4 * k + e] = q[e];
         }
+    }
+    return r;
+}
+template <int V, bool TAIL, typename T> __device__ __forceinline__ void widen_piece(Raw<V, T> r, int c0, int C, float* o) {
+    constexpr int PER = 4 / sizeof(T), W = V / PER;
+    if (TAIL && C >= V) {                                                     // the shift works on whole words, two 16-bit elements at a time
+        const int sh = c0 - min(c0, C - V);
 #pragma unroll
         for (int s = W / 2; s > 0; s /= 2)
 #pragma unroll
-            for (int e = 0; e < W; ++e) r[e] = (sh & (s * PER)) ? (e + s < W ? r[e + s] : 0u) : r[e];
+            for (int e = 0; e < W; ++e) r.w[e] = (sh & (s * PER)) ? (e + s < W ? r.w[e + s] : 0u) : r.w[e];
         if constexpr (PER == 2) {
             const unsigned bits = (sh & 1) * 16;
 #pragma unroll
-            for (int e = 0; e < W; ++e) r[e] = __builtin_amdgcn_alignbit(e + 1 < W ? r[e + 1] : 0u, r[e], bits);
+            for (int e = 0; e < W; ++e) r.w[e] = __builtin_amdgcn_alignbit(e + 1 < W ? r.w[e + 1] : 0u, r.w[e], bits);
         }
 #pragma unroll
-        for (int e = 0; e < W; ++e) r[e] = sh >= V ? 0u : r[e];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if constexpr (PER == 1) o[e] = __uint_as_float(r[e]);
-            else o[e] = widen(T{(unsigned short)(e % 2 ? r[e / 2] >> 16 : r[e / 2] & 0xffffu)});
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = c0 + e < C ? widen(at(row, off + c0)[e]) : 0.f;
+        for (int e = 0; e < W; ++e) r.w[e] = sh >= V ? 0u : r.w[e];
     }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        if constexpr (PER == 1) o[e] = __uint_as_float(r.w[e]);
+        else o[e] = widen(T{(unsigned short)(e % 2 ? r.w[e / 2] >> 16 : r.w[e / 2] & 0xffffu)});
+    }
+}
+template <int V, bool TAIL, typename T> __device__ __forceinline__ void load_piece(const T* row, int off, int c0, int C, float* o) {
+    widen_piece<V, TAIL>(raw_piece<V, TAIL>(row, off, c0, C), c0, C, o);
 }
 template <int V, bool TAIL, typename T> __device__ __forceinline__ void store_piece(T* row, int off, int c0, int C, const float* v) {
     if (c0 + V <= C) {

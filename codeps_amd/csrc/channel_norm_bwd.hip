@@ -32,12 +32,29 @@ __device__ __forceinline__ void put_columns(const float* acc, float* lds, float*
     }
 }
 
+// A row's tensors as they lie in memory.
+template <int V, int NCH, typename TX, typename TR, bool ROWS> struct Row {
+    Raw<V, TX> x[NCH], dh[NCH], g[ROWS ? NCH : 1];
+    Raw<V, TR> r[NCH], dy[NCH];
+    float4 st;                                       // mean and 1 / deviation of both norms
+};
+
 // SUMS false (rows of more than 4096 channels, blocks of more than 512 threads: 128 registers each): the column sums are left to a pass of their own
 // (channel_norm_columns_kernel), which gets the row's two sums of n'^T
+//
+// Loads of a row are issued together, before anything is widened.  AHEAD: those of the next row as well, before the current one's arithmetic -- where the
+// registers allow no more than two waves per SIMD anyway (20485 x 768 bf16 around an fp32 residual, item gate, forward and backward 117 -> 115 us, 1536
+// channels 203 -> 197 us); elsewhere it costs a wave (65536 x 1024 bf16 297 -> 340 us).  Three waves per SIMD (168 registers, 32 bytes per lane spilled)
+// for gates held over 16-bit rows: 32768 x 2048 315 us, with two 410 us; fp32 rows would spill more (16384 x 2048 565 -> 619 us).
+template <typename TX, typename TR, bool BLOCK, int GATE, bool SUMS> struct Form {
+    static constexpr bool held = BLOCK && SUMS && GATE == GATE_HELD, one_type = std::is_same<TX, TR>::value;
+    static constexpr bool ahead = held && !one_type;
+    static constexpr int threads = !SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS, waves = held && one_type && sizeof(TX) == 2 ? 3 : 1;
+};
 template <typename TX, typename TR, int NCH, bool BLOCK, bool TAIL, bool FULL, int GATE, bool SUMS>
-__global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void channel_norm_bwd_kernel(Args a) {
+__global__ __launch_bounds__((Form<TX, TR, BLOCK, GATE, SUMS>::threads), (Form<TX, TR, BLOCK, GATE, SUMS>::waves)) void channel_norm_bwd_kernel(Args a) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8, E = V * NCH;
-    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS;
+    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS, AHEAD = Form<TX, TR, BLOCK, GATE, SUMS>::ahead;
     __shared__ float red[2][32];
     __shared__ float lds[BLOCK ? 1 : WAVE_THREADS * E];
     int turn = 0;
@@ -90,43 +107,75 @@ __global__ __launch_bounds__(!SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS) void cha
                 }
             }
         }
-        for (long long i = (long long)slice * at_.rpb + at_.first; i + sub < a.rpi; i += (long long)S * at_.rpb) {
-            const size_t row = (size_t)item * a.rpi + i;                       // the wave's first row
-            float u[E], d[E];                                                  // u = n(x), d: the gradient that runs backward
+        const auto fetch = [&](size_t row) {                                   // the wave's first row
+            Row<V, NCH, TX, TR, ROWS> q;
             const TX* px = (const TX*)a.x + row * a.xp;
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) load_piece<V, TAIL>(px, ox, c0[j], C, u + j * V);
-            float mu, rho, nmu = 0.f, nrho = 1.f;
+            for (int j = 0; j < NCH; ++j) q.x[j] = raw_piece<V, TAIL>(px, ox, c0[j], C);
             if constexpr (!FULL) {
 #pragma unroll
-                for (int j = 0; j < NCH; ++j) load_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, odh, c0[j], C, d + j * V);
+                for (int j = 0; j < NCH; ++j) q.dh[j] = raw_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, odh, c0[j], C);
                 const float2 st = *reinterpret_cast<const float2*>(a.stats_in + (row + sub) * 2);
-                mu = st.x; rho = st.y;
-#pragma unroll
-                for (int k = 0; k < E; ++k) u[k] = (u[k] - mu) * rho;
+                q.st = make_float4(st.x, st.y, 0.f, 1.f);
             } else {
-                float t[E], y[E], al[ROWS ? E : 1], as[ROWS ? E : 1];          // dh; r, then u'; alpha act(g), alpha act'(g) of the row
-                const float4 st = *reinterpret_cast<const float4*>(a.stats_in + (row + sub) * 4);
-                mu = st.x; rho = st.y; nmu = st.z; nrho = st.w;
+                q.st = *reinterpret_cast<const float4*>(a.stats_in + (row + sub) * 4);
                 if constexpr (ROWS) {
 #pragma unroll
-                    for (int j = 0; j < NCH; ++j) load_piece<V, TAIL>((const TX*)a.gate + row * a.gp, og, c0[j], C, al + j * V);
+                    for (int j = 0; j < NCH; ++j) q.g[j] = raw_piece<V, TAIL>((const TX*)a.gate + row * a.gp, og, c0[j], C);
                 }
                 if (a.next) {
                     // without a residual x's row stands in for it (then both have one type) and counts as zeros: no branch around the load
                     const TR* pr = has_r ? (const TR*)a.r + row * a.rp : (const TR*)(const void*)px;
 #pragma unroll
                     for (int j = 0; j < NCH; ++j) {
-                        load_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, odh, c0[j], C, t + j * V);
-                        load_piece<V, TAIL>(pr, has_r ? orr : ox, c0[j], C, y + j * V);
+                        q.dh[j] = raw_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, odh, c0[j], C);
+                        q.r[j] = raw_piece<V, TAIL>(pr, has_r ? orr : ox, c0[j], C);
                     }
                 }
                 if (a.dy) {
 #pragma unroll
-                    for (int j = 0; j < NCH; ++j) load_piece<V, TAIL>((const TR*)a.dy + row * a.dyp, ody, c0[j], C, d + j * V);
-                } else {
+                    for (int j = 0; j < NCH; ++j) q.dy[j] = raw_piece<V, TAIL>((const TR*)a.dy + row * a.dyp, ody, c0[j], C);
+                }
+            }
+            return q;
+        };
+        const long long i0 = (long long)slice * at_.rpb + at_.first, step = (long long)S * at_.rpb;
+        Row<V, NCH, TX, TR, ROWS> now, ahead;
+        if constexpr (AHEAD) {
+            if (i0 + sub < a.rpi) ahead = fetch((size_t)item * a.rpi + i0);
+        }
+        for (long long i = i0; i + sub < a.rpi; i += step) {
+            const size_t row = (size_t)item * a.rpi + i;
+            if constexpr (AHEAD) {
+                now = ahead;
+                if (i + step + sub < a.rpi) ahead = fetch(row + step);
+            } else {
+                now = fetch(row);
+            }
+            float u[E], d[E];                                                  // u = n(x), d: the gradient that runs backward
 #pragma unroll
-                    for (int k = 0; k < E; ++k) d[k] = 0.f;
+            for (int j = 0; j < NCH; ++j) widen_piece<V, TAIL>(now.x[j], c0[j], C, u + j * V);
+            const float mu = now.st.x, rho = now.st.y, nmu = now.st.z, nrho = now.st.w;
+            if constexpr (!FULL) {
+#pragma unroll
+                for (int j = 0; j < NCH; ++j) widen_piece<V, TAIL>(now.dh[j], c0[j], C, d + j * V);
+#pragma unroll
+                for (int k = 0; k < E; ++k) u[k] = (u[k] - mu) * rho;
+            } else {
+                float t[E], y[E], al[ROWS ? E : 1], as[ROWS ? E : 1];          // dh; r, then u'; alpha act(g), alpha act'(g) of the row
+#pragma unroll
+                for (int j = 0; j < NCH; ++j) {
+                    if constexpr (ROWS) widen_piece<V, TAIL>(now.g[j], c0[j], C, al + j * V);
+                    if (a.next) {
+                        widen_piece<V, TAIL>(now.dh[j], c0[j], C, t + j * V);
+                        widen_piece<V, TAIL>(now.r[j], c0[j], C, y + j * V);
+                    }
+                    if (a.dy) {
+                        widen_piece<V, TAIL>(now.dy[j], c0[j], C, d + j * V);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) d[j * V + e] = 0.f;
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
@@ -347,15 +396,14 @@ __global__ __launch_bounds__(16 * FINISH_STREAMS) void channel_norm_finish_kerne
 }
 
 // Blocks: as many as are resident at once, by the registers of the kernel that runs -- more leave a tail of late blocks, fewer leave lanes idle.  Forward and
-// backward together at 8 / 12 / 16 / 20 waves per CU: 20485 x 768 bf16 in fp32, item gate 122 / 142 / 149 / - us; 32768 x 2048 bf16, channel gate 421 / 351 /
-// 429 / 395 us; 65536 x 1024 bf16, no gate 381 / 319 / 300 / 351 us; 524288 x 128 bf16, no gate 272 / 263 / 294 / 274 us; 65536 x 512 bf16, gate per
-// element 189 / 183 / 200 / 190 us; norm alone, 262144 x 128 fp32 at 16 / 20 / 28: 130 / 131 / 137 us.  A block takes at least 8 rows per row group where
-// there are that many: its column sums' slab is a cost of its own.
+// backward together at 8 / 12 / 16 waves per CU, us: norm alone, 65536 x 768 bf16 146 / 125 / 117, 16384 x 2048 fp32 131 / 133 / 140; block end in one 16-bit
+// type, 65536 x 1024 with an added norm 290 / 275 / 283, 32768 x 2048 with a channel gate 357 / 316 / 374; 16-bit blocks around an fp32 residual, 32768 x
+// 2048 389 / 396 / 424, 20485 x 768 with an item gate 115 / 128 / 133; all fp32, 20485 x 768 with an item gate 151 / 171 / 184, 32768 x 1024 274 / 279 / 292.
+// A block takes at least 8 rows per row group where there are that many: its column sums' slab is a cost of its own.
 Plan bwd_plan(const codeps_channel_norm_desc* d) {
     const Shape s = shape_of(d);
     const bool half = d->x_type != CODEPS_F32, held = d->gate_mode == CODEPS_GATE_CHANNEL || d->gate_mode == CODEPS_GATE_ITEM;
-    const int waves = !d->full ? 16 : held && (!s.block || d->res_type != d->x_type) && s.nch == (half ? 1 : 2) ? 8
-                    : d->gate_mode == CODEPS_GATE_NONE && s.block && half ? 16 : 12;
+    const int waves = !half || d->res_type != d->x_type ? 8 : !d->full ? 16 : held && !s.block ? 8 : 12;
     const int resident = CUS * std::max(1, waves / (s.threads / 64));
     return plan_of(d, (int)std::max<long long>(CUS, std::min<long long>(resident, d->rows / (8LL * s.rpb))), resident);
 }
