@@ -32,6 +32,7 @@ __device__ __forceinline__ void put_columns(const float* acc, float* lds, float*
     }
 }
 
+enum { SUMS_APART, SUMS_HERE, SUMS_WIDE };
 // A row's tensors as they lie in memory.
 template <int V, int NCH, typename TX, typename TR, bool ROWS> struct Row {
     Raw<V, TX> x[NCH], dh[NCH], g[ROWS ? NCH : 1];
@@ -39,22 +40,26 @@ template <int V, int NCH, typename TX, typename TR, bool ROWS> struct Row {
     float4 st;                                       // mean and 1 / deviation of both norms
 };
 
-// SUMS false (rows of more than 4096 channels, blocks of more than 512 threads: 128 registers each): the column sums are left to a pass of their own
-// (channel_norm_columns_kernel), which gets the row's two sums of n'^T
+// Rows of more than 4096 channels take blocks of more than 512 threads, which have 128 registers each.  SUMS_WIDE: the column sums fit there (norm alone, block
+// ends without a gate in one type): 4096 x 8192 bf16, norm alone, 108 us, forward and backward, with a pass of their own 139; 4096 x 5000 with residual and next
+// norm 175 / 204 us.  SUMS_APART: they would spill (16-bit rows around an fp32 residual 190 -> 212 us, a gate per element 190 -> 207, per channel 180 -> 263):
+// channel_norm_columns_kernel forms them from the row's two sums of n'^T.
 //
 // Loads of a row are issued together, before anything is widened.  AHEAD: those of the next row as well, before the current one's arithmetic -- where the
 // registers allow no more than two waves per SIMD anyway (20485 x 768 bf16 around an fp32 residual, item gate, forward and backward 117 -> 115 us, 1536
-// channels 203 -> 197 us); elsewhere it costs a wave (65536 x 1024 bf16 297 -> 340 us).  Three waves per SIMD (168 registers, 32 bytes per lane spilled)
-// for gates held over 16-bit rows: 32768 x 2048 315 us, with two 410 us; fp32 rows would spill more (16384 x 2048 565 -> 619 us).
-template <typename TX, typename TR, bool BLOCK, int GATE, bool SUMS> struct Form {
-    static constexpr bool held = BLOCK && SUMS && GATE == GATE_HELD, one_type = std::is_same<TX, TR>::value;
-    static constexpr bool ahead = held && !one_type;
-    static constexpr int threads = !SUMS ? 1024 : BLOCK ? 512 : WAVE_THREADS, waves = held && one_type && sizeof(TX) == 2 ? 3 : 1;
+// channels 203 -> 197 us), and for a norm alone in wide rows, where one block fills a CU (4096 x 8192 bf16 120 -> 108 us); elsewhere it costs a wave
+// (65536 x 1024 bf16 297 -> 340 us).  Three waves per SIMD (168 registers, 32 bytes per lane spilled) for gates held over 16-bit rows: 32768 x 2048 315 us,
+// with two 410 us; fp32 rows would spill more (16384 x 2048 565 -> 619 us).
+template <typename TX, typename TR, bool BLOCK, bool FULL, int GATE, int SUMS> struct Form {
+    static constexpr bool held = BLOCK && SUMS == SUMS_HERE && GATE == GATE_HELD, one_type = std::is_same<TX, TR>::value;
+    static constexpr bool ahead = (held && !one_type) || (SUMS == SUMS_WIDE && !FULL);
+    static constexpr int threads = SUMS != SUMS_HERE ? 1024 : BLOCK ? 512 : WAVE_THREADS, waves = held && one_type && sizeof(TX) == 2 ? 3 : 1;
 };
-template <typename TX, typename TR, int NCH, bool BLOCK, bool TAIL, bool FULL, int GATE, bool SUMS>
-__global__ __launch_bounds__((Form<TX, TR, BLOCK, GATE, SUMS>::threads), (Form<TX, TR, BLOCK, GATE, SUMS>::waves)) void channel_norm_bwd_kernel(Args a) {
+constexpr bool sums_fit(bool full, int gate, bool one_type) { return !full || (gate == GATE_NONE && one_type); }
+template <typename TX, typename TR, int NCH, bool BLOCK, bool TAIL, bool FULL, int GATE, int SUMS>
+__global__ __launch_bounds__((Form<TX, TR, BLOCK, FULL, GATE, SUMS>::threads), (Form<TX, TR, BLOCK, FULL, GATE, SUMS>::waves)) void channel_norm_bwd_kernel(Args a) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8, E = V * NCH;
-    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS, AHEAD = Form<TX, TR, BLOCK, GATE, SUMS>::ahead;
+    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS, AHEAD = Form<TX, TR, BLOCK, FULL, GATE, SUMS>::ahead;
     __shared__ float red[2][32];
     __shared__ float lds[BLOCK ? 1 : WAVE_THREADS * E];
     int turn = 0;
@@ -277,12 +282,12 @@ __global__ __launch_bounds__((Form<TX, TR, BLOCK, GATE, SUMS>::threads), (Form<T
     }
 }
 
-// The column sums alone, for rows of more than 4096 channels: a thread owns V channels of every row of its slice and forms D from the row's statistics and
+// The column sums alone, for SUMS_APART: a thread owns V channels of every row of its slice and forms D from the row's statistics and
 // sums.  Reads the row's tensors a second time (from the L2s and the memory-side cache where few rows lie between).
-template <typename TX, typename TR, bool TAIL, bool FULL, int GATE>
+template <typename TX, typename TR, bool TAIL, int GATE>
 __global__ __launch_bounds__(256) void channel_norm_columns_kernel(Args a) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8;
-    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS;
+    constexpr bool HELD = GATE == GATE_HELD, ROWS = GATE == GATE_ROWS;
     const int C = a.C, S = a.slices, slice = slice_of(blockIdx.x, S, a.shared_lines), c0 = (int)(blockIdx.y * 256 + threadIdx.x) * V;
     float w[V], b[V], nw[V], gv[V], gs[V], aw[V] = {}, ab[V] = {}, anw[V] = {}, anb[V] = {}, ag[V];
     load_vector<V>(a.w, a.wt, 0, c0, C, 1.f, w);
@@ -305,41 +310,34 @@ __global__ __launch_bounds__(256) void channel_norm_columns_kernel(Args a) {
             const TX* px = (const TX*)a.x + row * a.xp;
             float u[V], d[V];
             load_piece<V, TAIL>(px, 0, c0, C, u);
-            if constexpr (!FULL) {
-                load_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, 0, c0, C, d);
-                const float2 st = *reinterpret_cast<const float2*>(a.stats_in + row * 2);
+            const float4 st = *reinterpret_cast<const float4*>(a.stats_in + row * 4);
+            float t[V], y[V];
+            if constexpr (ROWS) load_piece<V, TAIL>((const TX*)a.gate + row * a.gp, 0, c0, C, gv);
+            if (a.next) {
+                load_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, 0, c0, C, t);
+                load_piece<V, TAIL>(has_r ? (const TR*)a.r + row * a.rp : (const TR*)(const void*)px, 0, c0, C, y);
+            }
+            if (a.dy) load_piece<V, TAIL>((const TR*)a.dy + row * a.dyp, 0, c0, C, d);
+            else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) u[e] = (u[e] - st.x) * st.y;
-            } else {
-                const float4 st = *reinterpret_cast<const float4*>(a.stats_in + row * 4);
-                float t[V], y[V];
-                if constexpr (ROWS) load_piece<V, TAIL>((const TX*)a.gate + row * a.gp, 0, c0, C, gv);
+                for (int e = 0; e < V; ++e) d[e] = 0.f;
+            }
+            const float2 s = a.next ? *reinterpret_cast<const float2*>(a.row_sums + row * 2) : make_float2(0.f, 0.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                u[e] = (u[e] - st.x) * st.y;
+                const float an = u[e] * w[e] + b[e];
+                float val = a.scale, slope = 0.f;
+                if constexpr (ROWS) { gate_both(gv[e], a.act, val, slope); val *= a.scale; }
+                if constexpr (HELD) { val = gv[e]; slope = gs[e]; }
                 if (a.next) {
-                    load_piece<V, TAIL>((const TX*)a.dh + row * a.dhp, 0, c0, C, t);
-                    load_piece<V, TAIL>(has_r ? (const TR*)a.r + row * a.rp : (const TR*)(const void*)px, 0, c0, C, y);
+                    y[e] = ((has_r ? y[e] : 0.f) + val * an - st.z) * st.w;
+                    anw[e] += t[e] * y[e];
+                    anb[e] += t[e];
+                    d[e] += st.w * (t[e] * nw[e] - s.x - y[e] * s.y);
                 }
-                if (a.dy) load_piece<V, TAIL>((const TR*)a.dy + row * a.dyp, 0, c0, C, d);
-                else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) d[e] = 0.f;
-                }
-                const float2 s = a.next ? *reinterpret_cast<const float2*>(a.row_sums + row * 2) : make_float2(0.f, 0.f);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    u[e] = (u[e] - st.x) * st.y;
-                    const float an = u[e] * w[e] + b[e];
-                    float val = a.scale, slope = 0.f;
-                    if constexpr (ROWS) { gate_both(gv[e], a.act, val, slope); val *= a.scale; }
-                    if constexpr (HELD) { val = gv[e]; slope = gs[e]; }
-                    if (a.next) {
-                        y[e] = ((has_r ? y[e] : 0.f) + val * an - st.z) * st.w;
-                        anw[e] += t[e] * y[e];
-                        anb[e] += t[e];
-                        d[e] += st.w * (t[e] * nw[e] - s.x - y[e] * s.y);
-                    }
-                    if constexpr (HELD) ag[e] += slope * an * d[e];
-                    d[e] *= val;
-                }
+                if constexpr (HELD) ag[e] += slope * an * d[e];
+                d[e] *= val;
             }
 #pragma unroll
             for (int e = 0; e < V; ++e) { aw[e] += d[e] * u[e]; ab[e] += d[e]; }
@@ -408,7 +406,11 @@ Plan bwd_plan(const codeps_channel_norm_desc* d) {
     return plan_of(d, (int)std::max<long long>(CUS, std::min<long long>(resident, d->rows / (8LL * s.rpb))), resident);
 }
 size_t slab_floats(const codeps_channel_norm_desc* d, const Plan& p) { return (size_t)p.blocks * 4 * d->channels; }
-size_t row_floats(const codeps_channel_norm_desc* d, const Plan& p) { return p.s.threads > 512 && d->next_kind ? (size_t)d->rows * 2 : 0; }
+bool columns_apart(const codeps_channel_norm_desc* d, const Shape& s) {
+    const int gate = d->gate_mode == CODEPS_GATE_NONE ? GATE_NONE : d->gate_mode == CODEPS_GATE_ELEMENT ? GATE_ROWS : GATE_HELD;
+    return s.threads > 512 && !sums_fit(d->full, gate, d->res_type == d->x_type);
+}
+size_t row_floats(const codeps_channel_norm_desc* d, const Plan& p) { return columns_apart(d, p.s) && d->next_kind ? (size_t)d->rows * 2 : 0; }
 size_t gate_floats(const codeps_channel_norm_desc* d, const Plan& p) {
     return d->gate_mode == CODEPS_GATE_CHANNEL || d->gate_mode == CODEPS_GATE_ITEM ? (size_t)p.items * p.slices * d->channels : 0;
 }
@@ -461,16 +463,19 @@ extern "C" int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const 
             using TR = decltype(tr);
             constexpr bool BLOCK = decltype(block)::value, TAIL = decltype(tail)::value, FULL = decltype(full)::value;
             constexpr int NCH = decltype(nch)::value, GATE = decltype(gmode)::value;
-            if constexpr (BLOCK) {
-                if (p.s.threads > 512) {
-                    hipLaunchKernelGGL((channel_norm_bwd_kernel<TX, TR, NCH, true, TAIL, FULL, GATE, false>), dim3(p.blocks), dim3(p.s.threads), 0, st, a);
-                    if (a.cols)
-                        hipLaunchKernelGGL((channel_norm_columns_kernel<TX, TR, TAIL, FULL, GATE>),
-                                           dim3(p.blocks, cdiv(d->channels, 256 * (sizeof(TX) == 4 ? 4 : 8))), dim3(256), 0, st, a);
-                    return;
+            if (BLOCK && p.s.threads > 512) {
+                if constexpr (BLOCK) {
+                    constexpr int SUMS = sums_fit(FULL, GATE, std::is_same<TX, TR>::value) ? SUMS_WIDE : SUMS_APART;
+                    hipLaunchKernelGGL((channel_norm_bwd_kernel<TX, TR, NCH, true, TAIL, FULL, GATE, SUMS>), dim3(p.blocks), dim3(p.s.threads), 0, st, a);
+                    if constexpr (SUMS == SUMS_APART) {
+                        if (a.cols)
+                            hipLaunchKernelGGL((channel_norm_columns_kernel<TX, TR, TAIL, GATE>),
+                                               dim3(p.blocks, cdiv(d->channels, 256 * (sizeof(TX) == 4 ? 4 : 8))), dim3(256), 0, st, a);
+                    }
                 }
+            } else {
+                hipLaunchKernelGGL((channel_norm_bwd_kernel<TX, TR, NCH, BLOCK, TAIL, FULL, GATE, SUMS_HERE>), dim3(p.blocks), dim3(p.s.threads), 0, st, a);
             }
-            hipLaunchKernelGGL((channel_norm_bwd_kernel<TX, TR, NCH, BLOCK, TAIL, FULL, GATE, true>), dim3(p.blocks), dim3(p.s.threads), 0, st, a);
         });
         CODEPS_CHECK_LAUNCH("channel_norm_bwd_kernel");
     }
