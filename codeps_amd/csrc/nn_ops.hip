@@ -301,6 +301,10 @@ __global__ __launch_bounds__(256) void bn_bwd_apply_kernel(const float* __restri
 // ---------------------------------------------------------------------------------- BatchNorm, multi-group launches
 // Several independent statistic groups (contiguous row ranges of one [rows][C] tensor, e.g. the six pose-net calls of
 // an adaptation step batched into one forward) handled by ONE launch per phase: blockIdx.z = group.
+// Running statistic after a batch: old (1 - momentum) + batch momentum, with one order of roundings wherever it is formed (left to the compiler, some kernels
+// fused the one product and some the other).
+__device__ __forceinline__ float bn_running(float old, float batch, float momentum) { return __builtin_fmaf(old, 1.f - momentum, momentum * batch); }
+
 struct BnGroups { int n; long long row0[8]; long long rows[8]; float inv_count[8]; };
 
 // partial (sum (x - s_g), sum (x - s_g)^2) with s_g = first row of the group: part[g][blk][2][C]
@@ -371,8 +375,8 @@ __global__ __launch_bounds__(256) void bn_finalize_mg_kernel(const float* __rest
         const float v = fmaxf(s2 / n - d * d, 0.f);
         mean[g * C + c] = m; var[g * C + c] = v; invstd[g * C + c] = rsqrtf(v + eps);
         if (upd) {
-            rm = rm * (1.f - momentum) + momentum * m;
-            rv = rv * (1.f - momentum) + momentum * (v * (n / fmaxf(n - 1.f, 1.f)));
+            rm = bn_running(rm, m, momentum);
+            rv = bn_running(rv, v * (n / fmaxf(n - 1.f, 1.f)), momentum);
         }
     }
     if (upd && sub == 0) { running_mean[c] = rm; running_var[c] = rv; }
@@ -423,8 +427,8 @@ __global__ __launch_bounds__(256) void bn_sync_combine_kernel(const float* __res
         mean[g * C + c] = m; var[g * C + c] = v; invstd[g * C + c] = rsqrtf(v + eps);
         if (upd) {
             const float n = gr.inv_count[g];                     // here: the GLOBAL element count of the group
-            rm = rm * (1.f - momentum) + momentum * m;
-            rv = rv * (1.f - momentum) + momentum * (v * (n / fmaxf(n - 1.f, 1.f)));
+            rm = bn_running(rm, m, momentum);
+            rv = bn_running(rv, v * (n / fmaxf(n - 1.f, 1.f)), momentum);
         }
     }
     if (upd) { running_mean[c] = rm; running_var[c] = rv; }
@@ -484,8 +488,8 @@ __global__ __launch_bounds__(1024) void bn_finalize_tiles_kernel(const float* __
                 t[0] = sh0 + d; t[C] = rsqrtf(v + eps); t[2 * C] = ga; t[3 * C] = be;
             }
             if (tab.run_mean && c < tab.c_real) {
-                tab.run_mean[c] = tab.run_mean[c] * (1.f - tab.momentum) + tab.momentum * (sh0 + d);
-                tab.run_var[c] = tab.run_var[c] * (1.f - tab.momentum) + tab.momentum * (v * (n / fmaxf(n - 1.f, 1.f)));
+                tab.run_mean[c] = bn_running(tab.run_mean[c], sh0 + d, tab.momentum);
+                tab.run_var[c] = bn_running(tab.run_var[c], v * (n / fmaxf(n - 1.f, 1.f)), tab.momentum);
             }
         }
     }
@@ -538,8 +542,8 @@ __global__ __launch_bounds__(256) void bn_apply_mg_kernel(const float* __restric
             float rm = run.mean[c], rv = run.var[c];
             for (int g = 0; g < gr.n; ++g) {
                 const float n = (float)gr.rows[g];
-                rm = rm * (1.f - run.momentum) + run.momentum * mean[g * C + c];
-                rv = rv * (1.f - run.momentum) + run.momentum * (run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)));
+                rm = bn_running(rm, mean[g * C + c], run.momentum);
+                rv = bn_running(rv, run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)), run.momentum);
             }
             run.mean[c] = rm; run.var[c] = rv;
         }
@@ -838,8 +842,8 @@ __global__ __launch_bounds__(256) void bn_relu_pool_fwd_kernel(const float* __re
             float rm = run.mean[c], rv = run.var[c];
             for (int g = 0; g < gr.n; ++g) {
                 const float n = (float)gr.rows[g];
-                rm = rm * (1.f - run.momentum) + run.momentum * mean[g * C + c];
-                rv = rv * (1.f - run.momentum) + run.momentum * (run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)));
+                rm = bn_running(rm, mean[g * C + c], run.momentum);
+                rv = bn_running(rv, run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)), run.momentum);
             }
             run.mean[c] = rm; run.var[c] = rv;
         }
@@ -2093,8 +2097,8 @@ __global__ __launch_bounds__(256) void bn_in_affine_kernel(const float* __restri
             float rm = run.mean[c], rv = run.var[c];
             for (int g = 0; g < ig.n; ++g) {
                 const float n = (float)((long long)(ig.b1[g] - ig.b0[g]) * rows_per_image);
-                rm = rm * (1.f - run.momentum) + run.momentum * mean[g * C + c];
-                rv = rv * (1.f - run.momentum) + run.momentum * (run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)));
+                rm = bn_running(rm, mean[g * C + c], run.momentum);
+                rv = bn_running(rv, run.batch_var[g * C + c] * (n / fmaxf(n - 1.f, 1.f)), run.momentum);
             }
             run.mean[c] = rm; run.var[c] = rv;
         }

@@ -209,3 +209,26 @@ def test_r50_bottleneck_stage_and_instance_decoder_with_and_without_deferral(ari
         F._DEFER = True
         lib().codeps_conv2d_set_arith(prev_arith)
         F.invalidate_weight_cache(True)
+
+
+@pytest.mark.parametrize("groups", [None, [(0, 1), (1, 2)]])
+def test_running_statistics_that_are_not_at_their_start_agree_bit_for_bit(groups):
+    """Three steps from arbitrary running statistics: the table's kernels, the apply pass and the plain statistics pass round in one order."""
+    from codeps_amd import functional as F
+    c = 64
+    g = torch.Generator().manual_seed(3)
+    start = torch.randn(c, generator=g), 0.5 + torch.rand(c, generator=g)
+    gamma, beta = torch.ones(c, device=DEV), torch.zeros(c, device=DEV)
+    w1, w2 = (torch.randn(c, 32, 3, 3, generator=g) * 0.1).to(DEV), (torch.randn(256, c, 1, 1, generator=g) * 0.1).to(DEV)
+    xs = [torch.randn(2, 64, 128, 32, generator=g).to(DEV) for _ in range(3)]
+    seen = []
+    for defer in (False, True):
+        rm, rv = (t.to(DEV) for t in start)
+        for x in xs:
+            z = F.conv2d(x, w1.clone().requires_grad_(True), pad=1, bn_stats=True)
+            y = F.batch_norm_train(z, gamma, beta, rm, rv, 0.1, 1e-5, act="relu", groups=groups, defer=defer)
+            assert (getattr(y, "_codeps_defer", None) is not None) == defer
+            F.conv2d(y, w2, exclusive=True)
+        torch.cuda.synchronize()
+        seen.append((rm, rv))
+    assert torch.equal(seen[0][0], seen[1][0]) and torch.equal(seen[0][1], seen[1][1])
