@@ -40,26 +40,25 @@ template <int V, int NCH, typename TX, typename TR, bool ROWS> struct Row {
     float4 st;                                       // mean and 1 / deviation of both norms
 };
 
-// Rows of more than 4096 channels take blocks of more than 512 threads, which have 128 registers each.  SUMS_WIDE: the column sums fit there (norm alone, block
-// ends without a gate in one type): 4096 x 8192 bf16, norm alone, 108 us, forward and backward, with a pass of their own 139; 4096 x 5000 with residual and next
-// norm 175 / 204 us.  SUMS_APART: they would spill (16-bit rows around an fp32 residual 190 -> 212 us, a gate per element 190 -> 207, per channel 180 -> 263):
+// Rows of more than 4096 channels take blocks of more than 512 threads, which have 128 registers each.  SUMS_WIDE: the column sums fit there (norm alone, 16-bit
+// block ends without a gate): 4096 x 8192 bf16, norm alone, 108 us, forward and backward, with a pass of their own 139; 4096 x 5000 with residual and next norm
+// 175 / 204 us.  SUMS_APART: they would spill (16-bit rows around an fp32 residual 190 -> 212 us, a gate per element 190 -> 207, per channel 180 -> 263):
 // channel_norm_columns_kernel forms them from the row's two sums of n'^T.
 //
-// Loads of a row are issued together, before anything is widened.  AHEAD: those of the next row as well, before the current one's arithmetic -- where the
-// registers allow no more than two waves per SIMD anyway (20485 x 768 bf16 around an fp32 residual, item gate, forward and backward 117 -> 115 us, 1536
-// channels 203 -> 197 us), and for a norm alone in wide rows, where one block fills a CU (4096 x 8192 bf16 120 -> 108 us); elsewhere it costs a wave
-// (65536 x 1024 bf16 297 -> 340 us).  Three waves per SIMD (168 registers, 32 bytes per lane spilled) for gates held over 16-bit rows: 32768 x 2048 315 us,
-// with two 410 us; fp32 rows would spill more (16384 x 2048 565 -> 619 us).
-template <typename TX, typename TR, bool BLOCK, bool FULL, int GATE, int SUMS> struct Form {
-    static constexpr bool held = BLOCK && SUMS == SUMS_HERE && GATE == GATE_HELD, one_type = std::is_same<TX, TR>::value;
-    static constexpr bool ahead = (held && !one_type) || (SUMS == SUMS_WIDE && !FULL);
-    static constexpr int threads = SUMS != SUMS_HERE ? 1024 : BLOCK ? 512 : WAVE_THREADS, waves = held && one_type && sizeof(TX) == 2 ? 3 : 1;
+// Loads of a row are issued together, before anything is widened.  AHEAD: those of the next row as well, before the current one's arithmetic: for gates held over
+// 16-bit rows, where the sums' registers allow two waves per SIMD either way (forward and backward: 20485 x 768 bf16 around an fp32 residual 117 -> 115 us,
+// 8192 x 4096 bf16 233 -> 214, 32768 x 2048 354 -> 336), and for a norm alone in wide rows, where one block fills a CU (4096 x 8192 bf16 120 -> 108 us).
+// Elsewhere it costs a wave (65536 x 1024 bf16 without gate 297 -> 340 us) or gains nothing (fp32 rows).
+template <typename TX, bool BLOCK, bool FULL, int GATE, int SUMS> struct Form {
+    static constexpr bool held = BLOCK && SUMS == SUMS_HERE && GATE == GATE_HELD;
+    static constexpr bool ahead = (held && sizeof(TX) == 2) || (SUMS == SUMS_WIDE && !FULL);
+    static constexpr int threads = SUMS != SUMS_HERE ? 1024 : BLOCK ? 512 : WAVE_THREADS;
 };
-constexpr bool sums_fit(bool full, int gate, bool one_type) { return !full || (gate == GATE_NONE && one_type); }
+constexpr bool sums_fit(bool full, int gate, bool all_16_bit) { return !full || (gate == GATE_NONE && all_16_bit); }
 template <typename TX, typename TR, int NCH, bool BLOCK, bool TAIL, bool FULL, int GATE, int SUMS>
-__global__ __launch_bounds__((Form<TX, TR, BLOCK, FULL, GATE, SUMS>::threads), (Form<TX, TR, BLOCK, FULL, GATE, SUMS>::waves)) void channel_norm_bwd_kernel(Args a) {
+__global__ __launch_bounds__((Form<TX, BLOCK, FULL, GATE, SUMS>::threads)) void channel_norm_bwd_kernel(Args a) {
     constexpr int V = sizeof(TX) == 4 ? 4 : 8, E = V * NCH;
-    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS, AHEAD = Form<TX, TR, BLOCK, FULL, GATE, SUMS>::ahead;
+    constexpr bool HELD = FULL && GATE == GATE_HELD, ROWS = FULL && GATE == GATE_ROWS, AHEAD = Form<TX, BLOCK, FULL, GATE, SUMS>::ahead;
     __shared__ float red[2][32];
     __shared__ float lds[BLOCK ? 1 : WAVE_THREADS * E];
     int turn = 0;
@@ -395,20 +394,20 @@ __global__ __launch_bounds__(16 * FINISH_STREAMS) void channel_norm_finish_kerne
 
 // Blocks: as many as are resident at once, by the registers of the kernel that runs -- more leave a tail of late blocks, fewer leave lanes idle.  Forward and
 // backward together at 8 / 12 / 16 waves per CU, us: norm alone, 65536 x 768 bf16 146 / 125 / 117, 16384 x 2048 fp32 131 / 133 / 140; block end in one 16-bit
-// type, 65536 x 1024 with an added norm 290 / 275 / 283, 32768 x 2048 with a channel gate 357 / 316 / 374; 16-bit blocks around an fp32 residual, 32768 x
-// 2048 389 / 396 / 424, 20485 x 768 with an item gate 115 / 128 / 133; all fp32, 20485 x 768 with an item gate 151 / 171 / 184, 32768 x 1024 274 / 279 / 292.
+// type, 65536 x 1024 with an added norm 290 / 275 / 283; 16-bit blocks around an fp32 residual, 32768 x 2048 389 / 396 / 424, 20485 x 768 with an item gate
+// 115 / 128 / 133; all fp32, 20485 x 768 with an item gate 151 / 171 / 184, 32768 x 1024 274 / 279 / 292.
 // A block takes at least 8 rows per row group where there are that many: its column sums' slab is a cost of its own.
 Plan bwd_plan(const codeps_channel_norm_desc* d) {
     const Shape s = shape_of(d);
     const bool half = d->x_type != CODEPS_F32, held = d->gate_mode == CODEPS_GATE_CHANNEL || d->gate_mode == CODEPS_GATE_ITEM;
-    const int waves = !half || d->res_type != d->x_type ? 8 : !d->full ? 16 : held && !s.block ? 8 : 12;
+    const int waves = !half || d->res_type != d->x_type ? 8 : !d->full ? 16 : held ? 8 : 12;
     const int resident = CUS * std::max(1, waves / (s.threads / 64));
     return plan_of(d, (int)std::max<long long>(CUS, std::min<long long>(resident, d->rows / (8LL * s.rpb))), resident);
 }
 size_t slab_floats(const codeps_channel_norm_desc* d, const Plan& p) { return (size_t)p.blocks * 4 * d->channels; }
 bool columns_apart(const codeps_channel_norm_desc* d, const Shape& s) {
     const int gate = d->gate_mode == CODEPS_GATE_NONE ? GATE_NONE : d->gate_mode == CODEPS_GATE_ELEMENT ? GATE_ROWS : GATE_HELD;
-    return s.threads > 512 && !sums_fit(d->full, gate, d->res_type == d->x_type);
+    return s.threads > 512 && !sums_fit(d->full, gate, d->x_type != CODEPS_F32 && d->res_type == d->x_type);
 }
 size_t row_floats(const codeps_channel_norm_desc* d, const Plan& p) { return columns_apart(d, p.s) && d->next_kind ? (size_t)d->rows * 2 : 0; }
 size_t gate_floats(const codeps_channel_norm_desc* d, const Plan& p) {
@@ -465,7 +464,7 @@ extern "C" int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const 
             constexpr int NCH = decltype(nch)::value, GATE = decltype(gmode)::value;
             if (BLOCK && p.s.threads > 512) {
                 if constexpr (BLOCK) {
-                    constexpr int SUMS = sums_fit(FULL, GATE, std::is_same<TX, TR>::value) ? SUMS_WIDE : SUMS_APART;
+                    constexpr int SUMS = sums_fit(FULL, GATE, sizeof(TX) == 2 && std::is_same<TX, TR>::value) ? SUMS_WIDE : SUMS_APART;
                     hipLaunchKernelGGL((channel_norm_bwd_kernel<TX, TR, NCH, true, TAIL, FULL, GATE, SUMS>), dim3(p.blocks), dim3(p.s.threads), 0, st, a);
                     if constexpr (SUMS == SUMS_APART) {
                         if (a.cols)
