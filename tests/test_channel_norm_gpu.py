@@ -465,3 +465,50 @@ def test_refusals():
     with pytest.raises(RuntimeError):                                 # no second derivative
         (g,) = torch.autograd.grad(F.channel_norm(leaf).sum(), [leaf], create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("gate", ["channel", "item", "element"])
+@pytest.mark.parametrize("dtype,res", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32)], ids=str)
+def test_activated_gates_at_the_ends_of_their_type(dtype, res, gate):
+    """Infinite gates and the largest finite ones are open or shut, and leave their neighbours alone: values and gradients of a sigmoid as everywhere (the 64-bit
+    one is exact there: 1 or 0, slope 0), a SiLU's gate is g where g is large and 0 at the type's lowest value; at +inf it is infinite, its own element alone.
+
+    1 / (1 + e^-g) is 0 once e^-g passes 2^126: the gate is off by at most |g| e^g < 2^7 2^-126 there (e^-g passes 2^150 at 104).  Behind it lie factors below
+    2^7 and sums of at most 80 of them: `floor`.  A SiLU's slope s (1 + g (1 - s)) passes through 0: it is off by at most 16 roundings of 2^-24 (its factors and
+    terms are below 1.3 where they matter, and take a dozen operations), whatever is left of it; the gate's gradient has that times |scale a da|, which `reference`
+    gives with the slope as a factor (and 64 or, in sums, 320 roundings)."""
+    C, floor = 72, 2.0 ** -126 * 2 ** 7 * 2 ** 7 * 80
+
+    def near(c, t, got):
+        d = {k: v.detach().double().cpu() for k, v in t.items()}
+        if gate == "item":
+            d["gate"] = d["gate"].reshape(rows[0], 1, C).expand(-1, math.prod(rows[1:]), -1)
+        want = reference(dict(c, items=rows[0]), {k: v if v.dim() == 1 else v.reshape(-1, C) for k, v in d.items()})
+        for k, g in got.items():
+            v, tol = want[k]
+            if k == "dgate":
+                slope = act_of(t["gate"].detach().double().cpu(), c["act"])[1].reshape(v.shape).abs()
+                tol = tol * (1 + 16 / (64 if gate == "element" else 320) / (slope + 2 * U))
+            assert torch.isfinite(g).all(), k
+            assert ((g.double().cpu().reshape(v.shape) - v).abs() <= half_step(g.dtype) * (v.abs() + tol) + tol + torch.finfo(g.dtype).tiny + floor).all(), k
+    for rows in ((5,), (2, 40)):
+        c = case(C, rows, dtype, res=res, gate=gate, act="sigmoid")
+        t = make(c, 5)
+        kept = t["gate"].dtype
+        ends = torch.tensor([math.inf, -math.inf, torch.finfo(kept).max, torch.finfo(kept).min, torch.finfo(kept).max / 1.2, torch.finfo(kept).max / 2, 89.0, -89.0],
+                            device=DEV).to(kept)
+        t["gate"][..., 3:3 + 8 * len(ends):8] = ends
+        near(c, t, run(c, t))
+        c = case(C, rows, dtype, res=res, gate=gate, act="silu", scale=2.0 ** -6, next=None)
+        t = make(c, 6)
+        for k in ("weight", "bias"):
+            t[k] *= 2.0 ** -6                                        # (so that the largest gates stay finite in y)
+        large = min(torch.finfo(v).max for v in (kept, dtype, res)) / 256
+        t["gate"][..., 3:51:8] = torch.tensor([torch.finfo(kept).min, large, 89.0, -89.0, 1000.0, -1000.0], device=DEV).to(kept)
+        clean = run(c, t)
+        near(c, t, clean)
+        t["gate"][..., 60] = math.inf
+        y = run(c, t)["y"]
+        a = F.channel_norm(t["x"].float(), t["weight"].float(), t["bias"].float(), eps=c["eps"])[..., 60]
+        keep = [i for i in range(C) if i != 60]
+        assert torch.equal(y[..., keep], clean["y"][..., keep]) and torch.equal(y[..., 60].float(), torch.where(a > 0, math.inf, -math.inf))
