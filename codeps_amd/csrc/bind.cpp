@@ -259,10 +259,16 @@ void check_vectors(Tensor& weight, Tensor& bias, double eps, const Tensor& x, co
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ Python calls
+// The kernels read addresses, and autograd's forward mode does not see that: the derivative would be dropped without a word.
+void check_forward_mode(const Tensor& t, const char* what) {
+    if (t._fw_grad(0).defined()) refuse(what, ": no forward-mode derivative (an input is a dual tensor)");
+}
 Tensor tensor_of(PyObject* o, const char* what) {
     if (o == Py_None) return Tensor();
     if (!THPVariable_Check(o)) refuse(what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    const Tensor& t = THPVariable_Unpack(o);
+    check_forward_mode(t, what);
+    return t;
 }
 void sinks_of(PyObject* o, Tensor (&sinks)[4]) {                      // None, or 4 tensors / Nones
     if (o == Py_None) return;
@@ -422,6 +428,7 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
             if (!THPVariable_Check(list[i])) refuse("grad_norm: tensors, got ", Py_TYPE(list[i])->tp_name);
             const Tensor& g = THPVariable_Unpack(list[i]);
             if (!first.defined()) first = g;
+            check_forward_mode(g, "grad_norm");
             check_gradient(g, first.device(), "grad_norm");
             if (dense(g)) {
                 ptrs.push_back(g.data_ptr());

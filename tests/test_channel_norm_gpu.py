@@ -512,3 +512,12 @@ def test_activated_gates_at_the_ends_of_their_type(dtype, res, gate):
         a = F.channel_norm(t["x"].float(), t["weight"].float(), t["bias"].float(), eps=c["eps"])[..., 60]
         keep = [i for i in range(C) if i != 60]
         assert torch.equal(y[..., keep], clean["y"][..., keep]) and torch.equal(y[..., 60].float(), torch.where(a > 0, math.inf, -math.inf))
+
+
+def test_transformed_tensors_are_refused():
+    """Dual tensors, and the wrappers of torch.func: an error, not an output without its derivative."""
+    x = torch.randn(5, 8, device=DEV)
+    for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.grad(lambda v: f(v).sum())(x), lambda f: torch.vmap(f)(x)):
+        for f in (F.channel_norm, lambda v: F.channel_norm_residual(v, x, next_kind="layer")[1], lambda v: F.channel_norm_residual(x, v), lambda v: F.grad_norm([v])):
+            with pytest.raises(RuntimeError):
+                transform(f)

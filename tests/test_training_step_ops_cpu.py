@@ -120,3 +120,17 @@ def test_struct_layouts():
     assert ctypes.sizeof(_lib.ChannelNormDesc) == 112 and _lib.ChannelNormDesc.channels.offset == 48 and _lib.ChannelNormDesc.scale.offset == 96
     assert ctypes.sizeof(_lib.StepBlock) == 19 * 8
     assert ctypes.sizeof(_lib.AdamWGroup) == 48 and _lib.AdamWGroup.lr_device.offset == 40
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Every tensor of a call, on its own: a dual tensor's derivative is not dropped silently (refused before the device is looked at)."""
+    import torch.autograd.forward_ad as forward
+    x, v = torch.ones(3, 4), torch.ones(4)
+    with forward.dual_level():
+        dx, dv = forward.make_dual(x, x), forward.make_dual(v, v)
+        for call in (lambda: F.channel_norm(dx), lambda: F.channel_norm(x, dv), lambda: F.channel_norm(x, v, dv), lambda: F.channel_norm_residual(dx),
+                     lambda: F.channel_norm_residual(x, dx), lambda: F.channel_norm_residual(x, gate=dv), lambda: F.channel_norm_residual(x, next_kind="rms", next_weight=dv),
+                     lambda: F.channel_norm_residual(x, next_kind="rms", next_weight=v, next_bias=dv), lambda: F.grad_norm([dx])):
+            for mode in (torch.enable_grad(), torch.no_grad()):
+                with mode, pytest.raises(CodepsHipError, match="forward-mode"):
+                    call()
