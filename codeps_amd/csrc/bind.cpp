@@ -422,6 +422,7 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
         std::vector<Tensor> copies;
         ptrs.reserve(list.size()); types.reserve(list.size()); numels.reserve(list.size());
         Tensor first;
+        const bool recording = at::GradMode::is_enabled();
         at::NoGradGuard off;
         for (Py_ssize_t i = 0; i < list.size(); ++i) {
             if (list[i] == Py_None) continue;
@@ -429,6 +430,8 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
             const Tensor& g = THPVariable_Unpack(list[i]);
             if (!first.defined()) first = g;
             check_forward_mode(g, "grad_norm");
+            if (recording && g.requires_grad())
+                refuse("grad_norm: the norm has no derivative and tensor ", i, " requires one: call it under torch.no_grad(), or detach them");
             check_gradient(g, first.device(), "grad_norm");
             if (dense(g)) {
                 ptrs.push_back(g.data_ptr());

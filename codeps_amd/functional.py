@@ -2396,7 +2396,8 @@ def adam_ema_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-4, betas=(0.9,
 
 def grad_norm(grads, scale=1.0):
     """|scale g|_2 over a list of gradients (None entries are skipped), fp32 on the device: what AdamW clips by (C ABI: codeps_grad_norm).  fp32, bf16 and
-    fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow."""
+    fp16 tensors may be mixed; the squares are summed in 64 bits in a fixed order, so the result does not change from run to run and does not overflow.
+    It has no derivative: tensors that require one (create_graph, weights) are taken under torch.no_grad() only."""
     return bind().grad_norm(grads, scale)
 
 

@@ -503,3 +503,17 @@ def test_tensors_that_move_between_steps(bits):
         a.step(iter(g + g))
     b.step(iter(g))                                                  # (any iterable serves)
     assert b.steps.tolist() == [7]
+
+
+def test_gradient_norm_of_gradients_with_a_graph():
+    """Refused while a graph is recorded, taken under no_grad; a step with such gradients is none of autograd's business either way."""
+    w = torch.nn.Parameter(torch.arange(1.0, 5.0, device=DEV))
+    (g,) = torch.autograd.grad((w ** 3).sum(), [w], create_graph=True)
+    with pytest.raises(CodepsHipError, match="no derivative"):
+        F.grad_norm([g])
+    with torch.no_grad():
+        norm = F.grad_norm([g, w])
+    want = math.sqrt(sum((3.0 * k * k) ** 2 + k * k for k in range(1, 5)))
+    assert not norm.requires_grad and abs(float(norm) - want) <= 2 * U * want
+    AdamW([w], lr=0.5, weight_decay=0.0).step([g])
+    assert torch.allclose(w.detach(), torch.arange(1.0, 5.0, device=DEV) - 0.5, rtol=0, atol=1e-5)

@@ -134,3 +134,16 @@ def test_forward_mode_derivatives_are_refused():
             for mode in (torch.enable_grad(), torch.no_grad()):
                 with mode, pytest.raises(CodepsHipError, match="forward-mode"):
                     call()
+
+
+def test_gradient_norm_of_tensors_that_require_a_gradient_is_refused():
+    """It would come back as a constant; under no_grad that is what is asked for (and the call goes on to the next check: the device)."""
+    plain, leaf = torch.ones(3), torch.nn.Parameter(torch.ones(3))
+    (graph,) = torch.autograd.grad((leaf ** 3).sum(), [leaf], create_graph=True)
+    for t in (leaf, graph):
+        with pytest.raises(CodepsHipError, match="no derivative"):
+            F.grad_norm([t, plain])
+        with torch.no_grad(), pytest.raises(CodepsHipError, match="GPU only"):
+            F.grad_norm([t, plain])
+        with pytest.raises(CodepsHipError, match="GPU only"):
+            F.grad_norm([t.detach(), plain])
