@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -263,6 +264,10 @@ void check_vectors(Tensor& weight, Tensor& bias, double eps, const Tensor& x, co
 void check_forward_mode(const Tensor& t, const char* what) {
     if (t._fw_grad(0).defined()) refuse(what, ": no forward-mode derivative (an input is a dual tensor)");
 }
+// torch.jit.trace does not see them either, and would keep the outputs of the example as constants.
+void check_trace(const char* what) {
+    if (at::tracer::impl::is_dispatch_enabled()) refuse(what, ": torch.jit.trace cannot record it");
+}
 Tensor tensor_of(PyObject* o, const char* what) {
     if (o == Py_None) return Tensor();
     if (!THPVariable_Check(o)) refuse(what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
@@ -309,6 +314,7 @@ PyObject* py_channel_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (!count(na, 6)) return nullptr;
     return guarded([&]() -> PyObject* {
         const char* what = "channel_norm";
+        check_trace(what);
         Norm n;
         n.x = tensor_of(a[0], what);
         if (!n.x.defined()) refuse(what, ": x is None");
@@ -333,6 +339,7 @@ PyObject* py_channel_norm_residual(PyObject*, PyObject* const* a, Py_ssize_t na)
     if (!count(na, 14)) return nullptr;
     return guarded([&]() -> PyObject* {
         const char* what = "channel_norm_residual";
+        check_trace(what);
         Norm n;
         auto& d = n.d;
         n.x = tensor_of(a[0], what);
@@ -414,6 +421,7 @@ void check_gradient(const Tensor& g, c10::Device device, const char* what) {
 PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (!count(na, 2)) return nullptr;
     return guarded([&]() -> PyObject* {
+        check_trace("grad_norm");
         const Sequence list(a[0]);
         const double scale = number(a[1]);
         std::vector<const void*> ptrs;
@@ -476,6 +484,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (!count(na, 8)) return nullptr;
     return guarded([&]() -> PyObject* {
         const char* what = "AdamW.step";
+        check_trace(what);
         const Sequence params(a[0]), beside(a[1]), grads(a[2]);
         const StepBlock* block = PyLong_Check(a[3]) ? (const StepBlock*)PyLong_AsVoidPtr(a[3]) : nullptr;
         const Py_ssize_t n = params.size();

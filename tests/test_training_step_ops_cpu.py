@@ -147,3 +147,15 @@ def test_gradient_norm_of_tensors_that_require_a_gradient_is_refused():
             F.grad_norm([t, plain])
         with pytest.raises(CodepsHipError, match="GPU only"):
             F.grad_norm([t.detach(), plain])
+
+
+def test_a_trace_is_refused():
+    """torch.jit.trace would keep the example's outputs as constants."""
+    x = torch.ones(3, 4)
+    for call in (F.channel_norm, lambda v: F.channel_norm_residual(v, v), lambda v: F.grad_norm([v])):
+        with pytest.raises(CodepsHipError, match="trace"):
+            torch.jit.trace(call, (x,))
+    with pytest.raises(CodepsHipError, match="trace"):
+        torch.jit.trace(lambda v: v + _lib.bind().adamw_step([v], [], [v], 0, 1.0, 0.0, False, 0.9), (x,))
+    with pytest.raises(CodepsHipError, match="GPU only"):             # (and nothing of it stays behind)
+        F.channel_norm(x)
