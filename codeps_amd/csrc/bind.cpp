@@ -518,9 +518,14 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
                              block->steps, block->exp_avg, block->exp_avg_sq, block->exp_avg_codes, block->exp_avg_exponents, block->root_codes,
                              block->root_exponents, grad_scale, max_norm, skip, block->norm, block->seed, ema_alpha, block->workspace,
                              (size_t)block->workspace_bytes, stream_of(first)), "codeps_adamw_step");
-        for (Py_ssize_t i = 0; i < n; ++i) {                          // saved tensors of a graph that is still to run backward must notice
-            const Tensor& p = THPVariable_Unpack(params[i]);
-            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        // what the kernel has rewritten: saved tensors of a graph that is still to run backward must notice, and packs of frozen weights are kept by version
+        const auto rewritten = [](const Tensor& t) {
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        };
+        for (Py_ssize_t i = 0; i < n; ++i) rewritten(THPVariable_Unpack(params[i]));
+        for (Py_ssize_t i = 0; i < beside.size(); ++i) {              // averages (fp32; left alone with ema_alpha < 0), 16-bit copies
+            const Tensor& t = THPVariable_Unpack(beside[i]);
+            if (ema_alpha >= 0.0 || t.scalar_type() != at::kFloat) rewritten(t);
         }
         return PyLong_FromLong(0);
     });

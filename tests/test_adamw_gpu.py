@@ -517,3 +517,36 @@ def test_gradient_norm_of_gradients_with_a_graph():
     assert not norm.requires_grad and abs(float(norm) - want) <= 2 * U * want
     AdamW([w], lr=0.5, weight_decay=0.0).step([g])
     assert torch.allclose(w.detach(), torch.arange(1.0, 5.0, device=DEV) - 0.5, rtol=0, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_averages_and_copies_are_seen_to_change(dtype):
+    """A graph that saved a working copy, or an average, and runs backward behind the step ends in autograd's error, as it does for a parameter; frozen convolution
+    weights that are averages or copies are packed anew; apply_ema False leaves averages, and what was saved of them, alone."""
+    w = torch.nn.Parameter(torch.randn(16, 16, 1, 1, device=DEV))
+    other = torch.nn.Parameter(torch.randn(5, device=DEV))
+    ema, copy_ = w.detach().clone(), w.detach().to(dtype)
+    opt = AdamW([other, w], lr=0.5, weight_decay=0.0, ema=[None, ema], ema_alpha=0.5, copies=[None, copy_])
+    x, leaf = torch.randn(1, 8, 8, 16, device=DEV), torch.ones(16, 16, 1, 1, device=DEV, requires_grad=True)
+    conv = lambda t: torch.einsum("bhwc,oc->bhwo", x.double().cpu(), t.detach().double().cpu()[:, :, 0, 0])            # noqa: E731
+    grads = [None, torch.ones_like(w)]
+    for apply_ema in (True, False):
+        saved = {"parameter": (leaf * w).sum(), "average": (leaf * ema).sum(), "copy": (leaf.to(dtype) * copy_).sum()}
+        before = [F.conv2d(x, t).clone() for t in (ema, copy_)]
+        versions = ema._version, copy_._version
+        opt.step(grads, apply_ema=apply_ema)
+        assert (ema._version > versions[0]) == apply_ema and copy_._version > versions[1]
+        for k, loss in saved.items():
+            if k == "average" and not apply_ema:
+                loss.backward()
+            else:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    loss.backward()
+        for t, y, moved in zip((ema, copy_), before, (apply_ema, True)):
+            now = F.conv2d(x, t)
+            assert float((now.double().cpu() - conv(t)).abs().max()) <= 1e-4 and torch.equal(now, y) != moved
+    fresh = torch.zeros(4, device=DEV)
+    with torch.inference_mode():
+        frozen = torch.zeros(4, device=DEV)                          # (an inference tensor has no version)
+    AdamW([fresh], ema=[frozen]).step([torch.ones(4, device=DEV)])
+    assert frozen.any()
