@@ -130,6 +130,8 @@ class AdamW:
         self._shapes = [p.shape for p in self.params]
         self._items = torch.zeros(n * lib().codeps_adamw_item_bytes(), dtype=torch.uint8, device=dev)
         self._by = [t for t in self._ema + self._copies if t is not None]
+        for t in self.params + self._by:                          # a replayed step rewrites them and no version tells: weight packs go by the epoch
+            t._codeps_volatile = True
         self._c_addresses = (ctypes.c_ulonglong * (n + len(self._by)))()
         self._fill_items()
         self._ws = torch.empty(lib().codeps_adamw_workspace_bytes(n), dtype=torch.uint8, device=dev)
@@ -175,7 +177,8 @@ class AdamW:
 
     def step(self, grads=None, *, grad_scale=1.0, apply_ema=True):
         """One update of every parameter that has a gradient.  grads: one tensor (or None) per parameter in the order of `params`; default: their .grad.
-        The others keep value, states and step count.  grad_scale multiplies the gradients (1 / world size after a summing all-reduce); apply_ema False
+        The others keep value, states and step count.  Behind the replay of a captured step, functional.invalidate_weight_cache() before eager convolutions with
+        these tensors.  grad_scale multiplies the gradients (1 / world size after a summing all-reduce); apply_ema False
         leaves the EMA tensors alone."""
         params = self.params
         grads = [p.grad for p in params] if grads is None else list(grads)

@@ -550,3 +550,25 @@ def test_averages_and_copies_are_seen_to_change(dtype):
         frozen = torch.zeros(4, device=DEV)                          # (an inference tensor has no version)
     AdamW([fresh], ema=[frozen]).step([torch.ones(4, device=DEV)])
     assert frozen.any()
+
+
+def test_a_replayed_step_is_seen_by_the_weight_packs():
+    """Parameters (trainable, and plain tensors with gradients of their own), averages and copies as convolution weights, before and behind replays."""
+    made = [torch.nn.Parameter(torch.randn(16, 16, 1, 1, device=DEV)), torch.randn(16, 16, 1, 1, device=DEV)]
+    ema, copies = [p.detach().clone() for p in made], [p.detach().to(BF16) for p in made]
+    opt = AdamW(made, lr=0.5, weight_decay=0.0, ema=ema, ema_alpha=0.5, copies=copies)
+    grads, x = [torch.ones_like(p) for p in made], torch.randn(1, 8, 8, 16, device=DEV)
+    opt.step(grads)
+    weights = made + ema + copies
+    seen = [F.conv2d(x, w).detach().clone() for w in weights]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(grads)
+    for _ in range(3):
+        graph.replay()
+        F.invalidate_weight_cache()
+        for i, w in enumerate(weights):
+            now = F.conv2d(x, w).detach().clone()
+            want = torch.einsum("bhwc,oc->bhwo", x.double().cpu(), w.detach().double().cpu()[:, :, 0, 0])
+            assert float((now.double().cpu() - want).abs().max()) <= 1e-4 and not torch.equal(now, seen[i]), i
+            seen[i] = now
