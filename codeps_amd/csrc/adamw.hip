@@ -14,7 +14,10 @@
 //   q = floor(t / quantum + rho / 65536),  rho = 16 random bits
 // in integers: t 2^16 / quantum is below 2^21, its whole part plus rho is shifted by 16.  The fp32 value behind it is off by a unit at most, so the
 // result can differ from the exact one only where the sum lies within two units of a multiple of 65536: there (about 8 elements in 100 000) the
-// moments are formed again in 64 bits.
+// moments are formed again in 64 bits.  The root is held over the whole range of fp32, but its square is not: a block goes through 64 bits as a whole, its unit
+// and the parameters' update included, where a square would overflow (roots of 2^62 or more) or lose bits that a code could see.  Those are squares below
+// 2^-120 that are not exactly zero, in blocks whose largest root is below 2^-36, or beside an eps below 2^-50: elsewhere, what a subnormal square loses (2^-74
+// of the root) is less than the 2^-16 quanta of the lowest codes (2^-70) and a rounding of the update's denominator.
 #include <algorithm>
 #include <type_traits>
 
@@ -46,8 +49,10 @@ struct Factors {                                // of one tensor and step, in th
     unsigned k0, k1;                            // random keys
     int live;                                   // 0: no gradient, or the step is skipped
     int skipped;                                // the whole step is (nothing changes, EMA included)
-    int pad;
+    int with64;                                 // WITH64_*
 };
+
+enum { WITH64_SCALE = 1, WITH64_ROOT = 2 };      // fp32 does not hold gs as a normal number | eps is too small to hide what a root below 2^-60 has lost
 
 struct Grads {                                  // launch argument: the gradients of up to PER_LAUNCH tensors
     const void* g[PER_LAUNCH];
@@ -211,14 +216,15 @@ __global__ __launch_bounds__(THREADS) void adamw_factors_kernel(Groups groups, c
         long long t = steps[base + i];
         if (live) steps[base + i] = ++t;
         Factors f;
-        f.live = live; f.skipped = skip; f.pad = 0;
+        f.live = live; f.skipped = skip;
         f.b1 = g.b1; f.ob1 = 1.0 - g.b1; f.b2 = g.b2; f.ob2 = 1.0 - g.b2; f.gs = gs;
         f.fb1 = (float)f.b1; f.fob1 = (float)f.ob1; f.fb2 = (float)f.b2; f.fob2 = (float)f.ob2; f.fgs = (float)gs;
-        const double lr = g.lr_dev ? (double)*g.lr_dev : g.lr;
+                const double lr = g.lr_dev ? (double)*g.lr_dev : g.lr;
         f.keep = (float)(1.0 - lr * g.wd);
         f.rate = (float)(lr / (1.0 - pow(g.b1, (double)t)));
         f.root = (float)(1.0 / sqrt(1.0 - pow(g.b2, (double)t)));
         f.eps = (float)g.eps;
+        f.with64 = (gs != 0.0 && !(fabs(gs) >= 0x1p-126 && fabs(gs) < 0x1p127) ? WITH64_SCALE : 0) | (f.eps >= f.root * 0x1p-50f ? 0 : WITH64_ROOT);
         unsigned long long z = seed + (unsigned long long)t * 0x9E3779B97F4A7C15ull + (unsigned long long)(base + i) * 0xD1B54A32D192ED03ull;
         z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
         z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
@@ -252,6 +258,11 @@ template <int MANT> __device__ __forceinline__ unsigned encode64(double a, int u
     const int low = a == 0.0 ? -14 : max(__builtin_amdgcn_frexp_exp(a) - 1 + 127 - unit, -14);
     const unsigned k = (unsigned)ldexp(a, 143 + MANT - unit - low) + rho;
     return min(((unsigned)(low + 14) << MANT) + (k >> 16), (16u << MANT) - 1u);
+}
+// unit_of in 64 bits
+template <int MANT> __device__ __forceinline__ unsigned unit64(double a) {
+    const unsigned e = (unsigned)(((unsigned long long)__double_as_longlong(a) + ((1ull << (52 - MANT)) - 1)) >> 52) - (1023 - 127);
+    return a < 0x1p-126 ? 0u : min(e, 255u);
 }
 __device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsigned k1) {
     unsigned x = (unsigned)i + (unsigned)(i >> 32) * 0x9E3779B1u + k0;
@@ -333,6 +344,7 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
             const float bad_m = um == 255 ? __uint_as_float(0x7fc00000u) : 0.f, bad_r = ur == 255 ? __uint_as_float(0x7fc00000u) : 0.f;
             float m0[4], r0[4], c[4];
             unsigned mtop = 0, rtop = 0;
+            bool deep = false;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned code = mc[k] >> (8 * e);
@@ -343,33 +355,59 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 c[e] = f.fob1 * gg;
                 a[k][e] = __builtin_fmaf(f.fb1, m0[e], c[e]);
                 b[k][e] = __builtin_amdgcn_sqrtf(__builtin_fmaf(f.fb2, r0[e] * r0[e], f.fob2 * gg * gg));
-                p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(b[k][e] * f.root + f.eps);
                 mtop = max(mtop, __float_as_uint(a[k][e]) & 0x7fffffffu);
                 rtop = max(rtop, __float_as_uint(b[k][e]) & 0x7fffffffu);
             }
-            const int nm = unit_of<MANT_M>(wave_umax(mtop)), nr = unit_of<MANT_R>(wave_umax(rtop));
-            const bool small = nm < 14 || nr < 14;                             // (a block of nearly nothing: all of it in 64 bits)
-            unsigned ncm = 0, ncr = 0;
+            int nm = unit_of<MANT_M>(wave_umax(mtop)), nr = unit_of<MANT_R>(wave_umax(rtop));
+            if (nr < 91 || (f.with64 & WITH64_ROOT)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned rnd = random_bits(i + e, f.k0, f.k1);
-                bool dm, dr;
-                // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
-                const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(c[e]);
-                const int low = place_of<MANT_M>(am, nm);
-                const unsigned slack = 2u + (unsigned)fminf(__builtin_ldexpf(size, 143 + MANT_M - 22 - nm - low), 33000.f);        // (2 * 33002 covers every remainder)
-                bool minus = a[k][e] < 0.f;
-                unsigned cm = encode<MANT_M>(am, nm, low, rnd & 0xffffu, slack, dm);
-                unsigned cr = encode<MANT_R>(b[k][e], nr, place_of<MANT_R>(b[k][e], nr), rnd >> 16, 2u, dr);
-                if (dm || dr || small) {
-                    double m, v;
-                    moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m, v);
-                    minus = m < 0.0;
-                    cm = encode64<MANT_M>(fabs(m), nm, rnd & 0xffffu);
-                    cr = encode64<MANT_R>(sqrt(v), nr, rnd >> 16);
+                for (int e = 0; e < 4; ++e) deep = deep || (b[k][e] < 0x1p-60f && (r0[e] != 0.f || g[k][e] != 0.f));
+                deep = __builtin_amdgcn_ballot_w64(deep) != 0;
+            }
+            unsigned ncm = 0, ncr = 0;
+            if (deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE)) {                // the same for the whole wave
+                double m[4], r[4];
+                unsigned tm = 0, tr = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    double v;
+                    moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m[e], v);
+                    r[e] = sqrt(v);
+                    p[k][e] = (float)((double)p[k][e] * f.keep - (double)f.rate * m[e] / (r[e] * f.root + f.eps));
+                    tm = max(tm, unit64<MANT_M>(fabs(m[e])));
+                    tr = max(tr, unit64<MANT_R>(r[e]));
                 }
-                ncm |= (cm | (minus ? 128u : 0u)) << (8 * e);
-                ncr |= cr << (8 * e);
+                nm = (int)wave_umax(tm);
+                nr = (int)wave_umax(tr);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned rnd = random_bits(i + e, f.k0, f.k1);
+                    ncm |= (encode64<MANT_M>(fabs(m[e]), nm, rnd & 0xffffu) | (m[e] < 0.0 ? 128u : 0u)) << (8 * e);
+                    ncr |= encode64<MANT_R>(r[e], nr, rnd >> 16) << (8 * e);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(b[k][e] * f.root + f.eps);
+                    const unsigned rnd = random_bits(i + e, f.k0, f.k1);
+                    bool dm, dr;
+                    // m may come out of a cancellation: its error is that of its two terms, (|b1 m| + |(1 - b1) g'|) 2^-22, in units of 2^-16 quanta
+                    const float am = fabsf(a[k][e]), size = fabsf(f.fb1 * m0[e]) + fabsf(c[e]);
+                    const int low = place_of<MANT_M>(am, nm);
+                    const unsigned slack = 2u + (unsigned)fminf(__builtin_ldexpf(size, 143 + MANT_M - 22 - nm - low), 33000.f);    // (2 * 33002 covers every remainder)
+                    bool minus = a[k][e] < 0.f;
+                    unsigned cm = encode<MANT_M>(am, nm, low, rnd & 0xffffu, slack, dm);
+                    unsigned cr = encode<MANT_R>(b[k][e], nr, place_of<MANT_R>(b[k][e], nr), rnd >> 16, 2u, dr);
+                    if (dm || dr) {
+                        double m, v;
+                        moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m, v);
+                        minus = m < 0.0;
+                        cm = encode64<MANT_M>(fabs(m), nm, rnd & 0xffffu);
+                        cr = encode64<MANT_R>(sqrt(v), nr, rnd >> 16);
+                    }
+                    ncm |= (cm | (minus ? 128u : 0u)) << (8 * e);
+                    ncr |= cr << (8 * e);
+                }
             }
             if (nm == 255) ncm = 0;
             if (nr == 255) ncr = 0;

@@ -211,7 +211,7 @@ class AdamW:
         F.invalidate_weight_cache()
 
     def moments_8bit(self):
-        """(m, sqrt(v)) that the 8-bit states stand for, exact in bf16: the 8-bit tensors one after another, without padding."""
+        """(m, sqrt(v)) that the 8-bit states stand for, exact in bf16 (down to its 2^-133): the 8-bit tensors one after another, without padding."""
         if not self._n8:
             raise CodepsHipError("AdamW.moments_8bit: no tensor has 8-bit states")
         m = torch.empty(self._n8, dtype=torch.bfloat16, device=self.device)

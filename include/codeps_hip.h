@@ -560,7 +560,7 @@ int codeps_adamw_step(const void* items, int n_items, const int* chunk_items, co
                       unsigned char* root_codes, unsigned char* root_exponents, double grad_scale, double max_norm, int skip_nonfinite,
                       float* norm, unsigned long long seed, double ema_alpha, void* workspace, size_t workspace_bytes,
                       codeps_stream_t stream);
-/* The values the 8-bit states stand for (exact in bf16), tensors packed without padding at their packed_offset: m and sqrt(v). */
+/* The values the 8-bit states stand for (exact in bf16 from a block's exponent byte of 12 on; below that their lowest codes lie under bf16's 2^-133), tensors packed without padding at their packed_offset: m and sqrt(v). */
 int codeps_adamw_moments_8bit(const void* items, int n_items, const int* chunk_items, long long n_chunks,
                               const unsigned char* exp_avg_codes, const unsigned char* exp_avg_exponents, const unsigned char* root_codes,
                               const unsigned char* root_exponents, void* exp_avg_bf16, void* root_bf16, codeps_stream_t stream);

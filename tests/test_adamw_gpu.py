@@ -572,3 +572,66 @@ def test_a_replayed_step_is_seen_by_the_weight_packs():
             want = torch.einsum("bhwc,oc->bhwo", x.double().cpu(), w.detach().double().cpu()[:, :, 0, 0])
             assert float((now.double().cpu() - want).abs().max()) <= 1e-4 and not torch.equal(now, seen[i]), i
             seen[i] = now
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("betas,eps", [((0.9, 0.999), 1e-8), ((0.0, 0.0), 1e-8), ((0.9, 0.999), 0.0)])
+def test_eight_bit_states_over_the_whole_range(betas, eps, dtype):
+    """Blocks from 2^-126 to 2^126: the root's square leaves fp32 at 2^-63 and 2^64.  Blocks of one size, blocks whose elements spread over 2^24, and blocks of one
+    large and 255 far smaller elements; codes, units, values and parameters as the 64-bit formula has them, over steps in which the sizes change places."""
+    gen = torch.Generator().manual_seed(13)
+    rows = []
+    for k in range(-126, 127, 3):
+        base = torch.sign(torch.randn(3, 256, generator=gen, dtype=torch.float64)) * (1 + torch.rand(3, 256, generator=gen, dtype=torch.float64)) / 2
+        base[1] *= 2.0 ** -(24 * torch.rand(256, generator=gen, dtype=torch.float64))
+        base[2] *= 2.0 ** -(3.0 * (k % 8))
+        base[2, 5] = 0.75
+        rows.append(torch.sign(base) * (base.abs() * 2.0 ** k).clamp(min=2.0 ** -130))            # (no zeros: with eps = 0 their update is 0 / 0)
+    sizes = torch.cat(rows)
+    params = tensors([sizes.numel(), 100], 4)
+    opt = AdamW(params, lr=1e-2, betas=betas, eps=eps, state_bits=8, small_numel=1, seed=21)
+    plain = Plain(params, [0.01, 0.01], [8, 8], 1e-2, betas, eps, seed=21)
+    small = gradients(params, 3)[1]
+    # A root that was rounded to 0 beside a moment of 2^100 sends a parameter beyond fp32's range, by the formula: infinite from then on.
+    gone = np.zeros(sizes.numel(), bool)
+    for order in (sizes, sizes, sizes.roll(3, 0), sizes.flip(0), sizes * 0 + 2.0 ** -30):
+        grads = [order.reshape(-1).float().to(dtype).to(DEV), small]
+        assert (grads[0] != 0).all() and torch.isfinite(grads[0]).all()
+        opt.step(grads)
+        plain.step(grads)
+        gone |= np.abs(plain.p[0]) > torch.finfo(F32).max
+        assert np.array_equal(~torch.isfinite(params[0]).cpu().numpy(), gone) and gone.mean() < 0.01
+        plain.pe[0][gone] = np.inf
+        check(opt, plain)
+        # handed out in bf16: every code is exact there but the lowest of blocks whose unit is below 2^-115, whose quanta (2^-18 of it) are below bf16's, 2^-133
+        for have, want in zip(opt.moments_8bit(), (np.concatenate(plain.m), np.sqrt(np.concatenate(plain.v)))):
+            assert torch.equal(have.cpu(), torch.from_numpy(want).to(BF16))
+            assert np.array_equal(have.double().cpu().numpy()[256 * 14 * 3:], want[256 * 14 * 3:]) or order is not sizes
+
+
+def test_units_of_both_moments_at_the_ends_of_fp32():
+    """As test_tiny_and_huge_moments, the root's half: zeros below 2^-126, its own unit down to there, NaN where the unit would be 2^128 -- and from there on only."""
+    p = tensors([1280], 1)[0]
+    g = torch.zeros(1280)
+    g[0], g[256], g[512], g[768], g[1024] = 1e-39, 1e-30, 1.0, 3.4e38, 3.1e38
+    opt = AdamW([p], lr=0.0, betas=(0.0, 0.0), state_bits=8, small_numel=1, weight_decay=0.0)
+    opt.step([g.to(DEV)])
+    assert opt.root_exponents.tolist() == [0, 127 - 100, 127, 255, 254] and opt.exp_avg_exponents.tolist() == [0, 127 - 100, 127, 255, 254]
+    m, r = (t.float().cpu() for t in opt.moments_8bit())
+    for v, step in ((m, 2.0 ** -3), (r, 2.0 ** -4)):
+        assert float(v[0]) == 0.0 and float(v[512]) == 1.0 and torch.isnan(v[768:1024]).all() and not v[1:256].any()
+        assert abs(float(v[256]) / 1e-30 - 1) <= step and abs(float(v[1024]) / 3.1e38 - 1) <= step
+
+
+def test_one_huge_gradient_leaves_its_block_alone():
+    """A gradient whose square overflows fp32, for one step: what it leaves is finite, and the block goes on as the formula does."""
+    params = tensors([1024], 2)
+    opt, plain = AdamW(params, lr=1e-3, state_bits=8, small_numel=1, seed=3), Plain(params, [0.01], [8], 1e-3, (0.9, 0.999), 1e-8, seed=3)
+    for k in range(3):
+        grads = gradients(params, 60 + k)
+        if k == 0:
+            grads[0][300], grads[0][600] = 1e21, -3e38
+        opt.step(grads)
+        plain.step(grads)
+        check(opt, plain)
+        assert torch.isfinite(params[0]).all() and 255 not in opt.root_exponents.tolist()
