@@ -14,7 +14,8 @@
 //   q = floor(t / quantum + rho / 65536),  rho = 16 random bits
 // in integers: t 2^16 / quantum is below 2^21, its whole part plus rho is shifted by 16.  The fp32 value behind it is off by a unit at most, so the
 // result can differ from the exact one only where the sum lies within two units of a multiple of 65536: there (about 8 elements in 100 000) the
-// moments are formed again in 64 bits.  The root is held over the whole range of fp32, but its square is not: a block goes through 64 bits as a whole, its unit
+// moments are formed again in 64 bits.  So are those of a whole block whose largest magnitude lies next to a border between two units (about one block in
+// 100 000).  The root is held over the whole range of fp32, but its square is not: a block goes through 64 bits as a whole, its unit
 // and the parameters' update included, where a square would overflow (roots of 2^62 or more) or lose bits that a code could see.  Those are squares below
 // 2^-120 that are not exactly zero, in blocks whose largest root is below 2^-36, or beside an eps below 2^-50: elsewhere, what a subnormal square loses (2^-74
 // of the root) is less than the 2^-16 quanta of the lowest codes (2^-70) and a rounding of the update's denominator.
@@ -259,6 +260,10 @@ template <int MANT> __device__ __forceinline__ unsigned encode64(double a, int u
     const unsigned k = (unsigned)ldexp(a, 143 + MANT - unit - low) + rho;
     return min(((unsigned)(low + 14) << MANT) + (k >> 16), (16u << MANT) - 1u);
 }
+// whether a magnitude that is off by `steps` of its last place at most could have another unit
+template <int MANT> __device__ __forceinline__ bool next_to_border(unsigned top, unsigned steps) {
+    return ((top + ((1u << (23 - MANT)) - 1) + steps) & 0x7fffffu) <= 2 * steps;
+}
 // unit_of in 64 bits
 template <int MANT> __device__ __forceinline__ unsigned unit64(double a) {
     const unsigned e = (unsigned)(((unsigned long long)__double_as_longlong(a) + ((1ull << (52 - MANT)) - 1)) >> 52) - (1023 - 127);
@@ -358,14 +363,19 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 mtop = max(mtop, __float_as_uint(a[k][e]) & 0x7fffffffu);
                 rtop = max(rtop, __float_as_uint(b[k][e]) & 0x7fffffffu);
             }
-            int nm = unit_of<MANT_M>(wave_umax(mtop)), nr = unit_of<MANT_R>(wave_umax(rtop));
-            if (nr < 91 || (f.with64 & WITH64_ROOT)) {
+            mtop = wave_umax(mtop);
+            rtop = wave_umax(rtop);
+            int nm = unit_of<MANT_M>(mtop), nr = unit_of<MANT_R>(rtop);
+            // The largest magnitudes are off by 2^-21 of the root and 2^-21 of m's terms.  Those are below |m| + 2 |b1 m0|, and m0 below 2 of its block's units: at most
+            // 32 steps of m's last place, and twice as many for every binary place by which m has come out below m0's unit.
+            const bool unsure = next_to_border<MANT_M>(mtop, 32u << min(max(um + 1 - (int)(mtop >> 23), 0), 17)) || next_to_border<MANT_R>(rtop, 16u);
+            if (__builtin_expect(nr < 91 || (f.with64 & WITH64_ROOT), false)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) deep = deep || (b[k][e] < 0x1p-60f && (r0[e] != 0.f || g[k][e] != 0.f));
                 deep = __builtin_amdgcn_ballot_w64(deep) != 0;
             }
             unsigned ncm = 0, ncr = 0;
-            if (deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE)) {                // the same for the whole wave
+            if (__builtin_expect(unsure || deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE), false)) {                // the same for the whole wave
                 double m[4], r[4];
                 unsigned tm = 0, tr = 0;
 #pragma unroll
@@ -398,7 +408,7 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                     bool minus = a[k][e] < 0.f;
                     unsigned cm = encode<MANT_M>(am, nm, low, rnd & 0xffffu, slack, dm);
                     unsigned cr = encode<MANT_R>(b[k][e], nr, place_of<MANT_R>(b[k][e], nr), rnd >> 16, 2u, dr);
-                    if (dm || dr) {
+                    if (__builtin_expect(dm || dr, false)) {
                         double m, v;
                         moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m, v);
                         minus = m < 0.0;

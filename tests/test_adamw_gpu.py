@@ -575,7 +575,7 @@ def test_a_replayed_step_is_seen_by_the_weight_packs():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
-@pytest.mark.parametrize("betas,eps", [((0.9, 0.999), 1e-8), ((0.0, 0.0), 1e-8), ((0.9, 0.999), 0.0)])
+@pytest.mark.parametrize("betas,eps", [((0.9, 0.999), 1e-8), ((0.0, 0.0), 1e-8), ((0.9, 0.999), 0.0), ((0.5, 0.9999999), 1e-30)])
 def test_eight_bit_states_over_the_whole_range(betas, eps, dtype):
     """Blocks from 2^-126 to 2^126: the root's square leaves fp32 at 2^-63 and 2^64.  Blocks of one size, blocks whose elements spread over 2^24, and blocks of one
     large and 255 far smaller elements; codes, units, values and parameters as the 64-bit formula has them, over steps in which the sizes change places."""
@@ -635,3 +635,43 @@ def test_one_huge_gradient_leaves_its_block_alone():
         plain.step(grads)
         check(opt, plain)
         assert torch.isfinite(params[0]).all() and 255 not in opt.root_exponents.tolist()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_units_next_to_their_borders(dtype):
+    """Blocks whose largest moment, or root, falls within a few roundings of the border between two units, from states and gradients chosen for it: 64 bits decide.
+    One of them, m = 0.9 * -0.125 + 0.1 * 10.5, is 0.93749999999999978 in 64 bits and 0.9375000596 in 32, on both sides of a border."""
+    b1, b2, blocks = 0.9, 0.999, 1500
+    rng = np.random.default_rng(17)
+    gm, gr = np.array(grid(3)), np.array(grid(4))
+    n = 2 * blocks * 256
+    cm, cr, g = rng.integers(0, 60, n).astype(np.uint8), rng.integers(0, 100, n).astype(np.uint8), 1e-6 * rng.standard_normal(n)
+    near = torch.float32 if dtype is F32 else BF16
+
+    def rounded(v, steps):                                           # v in the gradient's type, `steps` of its last place further
+        t = torch.tensor(v, dtype=torch.float64).to(near)
+        return float(t) + steps * float(t.abs()) * torch.finfo(near).eps / 2
+    for b in range(2 * blocks):
+        at, border = 256 * b + int(rng.integers(256)), 2.0 ** int(rng.integers(-3, 4))
+        step = int(rng.integers(-2, 3)) if dtype is F32 else 0
+        if b < blocks:                                               # the first moment, often out of a cancellation
+            cm[at] = rng.integers(60, 127)
+            sign = -1.0 if rng.random() < 0.5 else 1.0
+            cm[at] |= 128 if sign < 0 else 0
+            g[at] = rounded(((2 - 2.0 ** -3) * border - b1 * sign * gm[cm[at] & 127]) / (1 - b1), step)
+        else:
+            cr[at] = rng.integers(100, 200)
+            g[at] = rounded(math.sqrt(max(((2 - 2.0 ** -4) * border) ** 2 - b2 * gr[cr[at]] ** 2, 1.0) / (1 - b2)), step)
+    cm[0], g[0] = 128 + (12 << 3), 10.5
+    grads = [torch.from_numpy(g).to(dtype).to(DEV)]
+    params = [torch.zeros(n, device=DEV)]
+    opt, plain = AdamW(params, lr=1e-3, betas=(b1, b2), state_bits=8, seed=2), Plain(params, [0.01], [8], 1e-3, (b1, b2), 1e-8, seed=2)
+    opt.exp_avg_codes.copy_(torch.from_numpy(cm))
+    opt.root_codes.copy_(torch.from_numpy(cr))
+    opt.exp_avg_exponents.fill_(127)
+    opt.root_exponents.fill_(127)
+    plain.m[0][:] = np.where(cm >= 128, -1, 1) * gm[cm & 127]
+    plain.v[0][:] = gr[cr] ** 2
+    opt.step(grads)
+    plain.step(grads)
+    check(opt, plain)
