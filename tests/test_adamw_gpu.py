@@ -675,3 +675,35 @@ def test_units_next_to_their_borders(dtype):
     opt.step(grads)
     plain.step(grads)
     check(opt, plain)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_beside_the_tensors_is_written(bits):
+    """Parameters, averages and copies as views of flat buffers with an element in front of, between and behind them, which keep their values; so do the states of
+    tensors without a gradient, between the others'."""
+    sizes = [1, 3, 255, 257, 2047, 2049, 700, 5000]
+    total, mark = sum(sizes) + len(sizes) + 1, 0.7109375                     # (exact in 16 bits)
+    flats = [torch.full((total,), mark, device=DEV), torch.full((total,), mark, device=DEV), torch.full((total,), mark, dtype=BF16, device=DEV)]
+    starts = [1 + sum(sizes[:i]) + i for i in range(len(sizes))]
+    cut = lambda flat: [flat[a:a + n] for a, n in zip(starts, sizes)]                              # noqa: E731
+    guard = torch.ones(total, dtype=torch.bool, device=DEV)
+    for a, n in zip(starts, sizes):
+        guard[a:a + n] = False
+    assert int(guard.sum()) == len(sizes) + 1
+    params, ema, copies = map(cut, flats)
+    opt = AdamW(params, lr=1e-2, state_bits=bits, small_numel=1, ema=ema, copies=copies, max_norm=1.0, seed=5)
+    for k in range(3):
+        grads = [None if k and i % 3 == 1 else g for i, g in enumerate(gradients(params, 40 + k, BF16))]
+        held = {n: t.clone() for n, t in zip(opt._STATES[1:], opt._states()) if t is not None}
+        opt.step(grads)
+        for flat in flats:
+            assert (flat[guard] == mark).all() and (flat[~guard] != mark).any()
+        for name, old in held.items():
+            unit = 256 if name.endswith("exponents") else 1
+            for off, n, g in zip(opt._offsets, sizes, grads):
+                a, b = off // unit, (off + (n if bits == 32 else -(-n // 256) * 256)) // unit
+                assert g is not None or torch.equal(old[a:b], getattr(opt, name)[a:b]), (name, n)
+    if bits == 8:                                                    # (the padding of a tensor's last block holds zeros)
+        for off, n in zip(opt._offsets, sizes):
+            end = off + -(-n // 256) * 256
+            assert not (opt.exp_avg_codes[off + n:end] & 127).any() and not opt.root_codes[off + n:end].any()
