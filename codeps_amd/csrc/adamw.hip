@@ -330,13 +330,23 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) grad4<TAIL>(gp, gt, first + k * THREADS * 4, n, g[k]);
+    float fgs = f.fgs;
+    if constexpr (WIDE) {
+        if (__builtin_expect(f.with64 & WITH64_SCALE, false)) {                // (clipping gradients of 1e38: the factor has few bits in fp32, or none)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[k][e] = (float)((double)g[k][e] * f.gs);
+            fgs = 1.f;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const long long i = first + k * THREADS * 4;
         if constexpr (WIDE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float gg = g[k][e] * f.fgs;
+                const float gg = g[k][e] * fgs;
                 a[k][e] = f.fb1 * a[k][e] + f.fob1 * gg;
                 b[k][e] = f.fb2 * b[k][e] + f.fob2 * gg * gg;
                 p[k][e] = p[k][e] * f.keep - f.rate * a[k][e] * __builtin_amdgcn_rcpf(sqrtf(b[k][e]) * f.root + f.eps);
@@ -356,7 +366,7 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 const float q = decode<MANT_M>(code & 127u, um) + bad_m;
                 m0[e] = __uint_as_float(__float_as_uint(q) | (code & 128u) << 24);
                 r0[e] = decode<MANT_R>(rc[k] >> (8 * e) & 255u, ur) + bad_r;
-                const float gg = g[k][e] * f.fgs;
+                const float gg = g[k][e] * fgs;
                 c[e] = f.fob1 * gg;
                 a[k][e] = __builtin_fmaf(f.fb1, m0[e], c[e]);
                 b[k][e] = __builtin_amdgcn_sqrtf(__builtin_fmaf(f.fb2, r0[e] * r0[e], f.fob2 * gg * gg));

@@ -707,3 +707,17 @@ def test_nothing_beside_the_tensors_is_written(bits):
         for off, n in zip(opt._offsets, sizes):
             end = off + -(-n // 256) * 256
             assert not (opt.exp_avg_codes[off + n:end] & 127).any() and not opt.root_codes[off + n:end].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_clipping_by_a_factor_below_fp32s_normal_range(bits, dtype):
+    """Gradients near fp32's largest, clipped to a small norm: the factor, 1e-41, has a few bits in fp32; the scaled gradients are ordinary numbers."""
+    params = tensors([1000, 300], 5)
+    opt = AdamW(params, lr=1e-2, state_bits=bits, small_numel=1, max_norm=1e-2, seed=7)
+    plain = Plain(params, [0.01] * 2, [bits] * 2, 1e-2, (0.9, 0.999), 1e-8, 1e-2, seed=7)
+    for k in range(2):
+        grads = [(g.double() / g.double().abs().max() * 3e38).to(dtype) for g in gradients(params, 70 + k)]
+        opt.step(grads)
+        plain.step(grads)
+        check(opt, plain)
