@@ -64,8 +64,10 @@ std::string described(const Tensor& t) { return c10::str(t.sizes(), " ", t.scala
 // ------------------------------------------------------------------------------------------------------------------------ channel norms
 constexpr int64_t MAX_CHANNELS = 8192, MAX_PITCH = 1 << 24;
 
-// t itself when its channels are dense and its rows lie at one distance (elements, in `pitch`), else a contiguous copy
-Tensor pitched(const Tensor& t, int64_t& pitch) {
+// t itself when its channels are dense and its rows lie at one distance (elements, in `pitch`), else a contiguous copy.  (A view that negates on reading --
+// the imaginary part of a conjugate -- holds the other sign in memory.)
+Tensor pitched(const Tensor& given, int64_t& pitch) {
+    const Tensor t = given.is_neg() ? given.resolve_neg() : given;
     const int64_t c = t.size(-1);
     pitch = c;
     if (t.is_contiguous()) return t;
@@ -253,6 +255,7 @@ void check_vectors(Tensor& weight, Tensor& bias, double eps, const Tensor& x, co
         if (!v->defined()) continue;
         if (v->dim() != 1 || v->size(0) != x.size(-1) || type_of(*v) < 0 || v->device() != x.device())
             refuse(what, ": weight and bias have one value per channel (", x.size(-1), ") in fp32, bf16 or fp16 on ", x.device(), ", got ", described(*v));
+        if (v->is_neg()) *v = v->resolve_neg();
         if (!v->is_contiguous()) *v = v->contiguous();
     }
     if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type())
@@ -505,7 +508,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t na) {
             const Tensor& g = THPVariable_Unpack(grads[i]);
             check_gradient(g, p.device(), what);
             if (g.sizes() != p.sizes()) refuse(what, ": gradient ", i, " is ", g.sizes(), ", its parameter ", p.sizes());
-            mixed = mixed || !dense(p) || !(g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous()));
+            mixed = mixed || g.is_neg() || !dense(p) || !(g.strides() == p.strides() || (g.is_contiguous() && p.is_contiguous()));
             ptrs[i] = g.numel() ? g.data_ptr() : (const void*)16;                      // (an empty tensor has no address, but a gradient)
             types[i] = (unsigned char)type_of(g);
         }

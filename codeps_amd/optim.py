@@ -84,8 +84,8 @@ class AdamW:
             require_cuda(p)
             if p.dtype != torch.float32 or p.device != dev:
                 raise CodepsHipError(f"AdamW: fp32 parameters on one device, got {p.dtype} on {p.device} (16-bit weights: `copies` of fp32 ones)")
-            if not _dense(p):
-                raise CodepsHipError(f"AdamW: a parameter of shape {tuple(p.shape)} with strides {p.stride()} is not dense")
+            if not _dense(p) or p.is_neg():
+                raise CodepsHipError(f"AdamW: a parameter of shape {tuple(p.shape)} with strides {p.stride()} is not dense, or is a view that negates")
             if p.numel() and p.data_ptr() in seen:
                 raise CodepsHipError("AdamW: a parameter is listed twice")
             seen.add(p.data_ptr())
@@ -145,7 +145,7 @@ class AdamW:
         if len(tensors) != len(self.params):
             raise CodepsHipError(f"AdamW: {what}: one entry per parameter ({len(self.params)}), got {len(tensors)}")
         for p, t in zip(self.params, tensors):
-            if t is not None and (t.dtype not in dtypes or t.device != self.device or not _same_layout(t, p)):
+            if t is not None and (t.dtype not in dtypes or t.device != self.device or not _same_layout(t, p) or t.is_neg()):
                 raise CodepsHipError(f"AdamW: {what}: {tuple(t.shape)} {t.dtype} on {t.device} does not go with a parameter of {tuple(p.shape)}")
         return tensors
 
@@ -205,7 +205,7 @@ class AdamW:
             if not all(map(_dense, params)):
                 raise CodepsHipError("AdamW.step: a parameter has changed its layout since it was listed")
             with torch.no_grad():
-                grads = [g if g is None or _same_layout(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
+                grads = [g if g is None or _same_layout(g, p) and not g.is_neg() else torch.empty_like(p, dtype=g.dtype).copy_(g) for g, p in zip(grads, params)]
         if state and bind().adamw_step(params, self._by, grads, *rest):
             raise CodepsHipError("AdamW.step: a parameter or gradient changes under the step")
         F.invalidate_weight_cache()

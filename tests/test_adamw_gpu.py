@@ -721,3 +721,18 @@ def test_clipping_by_a_factor_below_fp32s_normal_range(bits, dtype):
         opt.step(grads)
         plain.step(grads)
         check(opt, plain)
+
+
+def test_gradients_that_negate_on_reading():
+    """The imaginary part of a conjugate: the sign in memory is not the value's (one element has no strides that would have it copied)."""
+    for n in (1, 7):
+        z = torch.arange(1.0, n + 1, device=DEV).to(torch.complex64)
+        g = (1j * z).conj().imag
+        p, q = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+        assert g.is_neg() and float(g[0]) == -1.0
+        AdamW([p], lr=0.5, weight_decay=0.0).step([g])
+        AdamW([q], lr=0.5, weight_decay=0.0).step([g.clone()])
+        assert torch.equal(p, q) and (p > 0).all()
+        for bad in (lambda: AdamW([g[:1]]), lambda: AdamW([p[:1]], ema=[g[:1]])):
+            with pytest.raises(CodepsHipError):
+                bad()

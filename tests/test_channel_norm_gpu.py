@@ -521,3 +521,22 @@ def test_transformed_tensors_are_refused():
         for f in (F.channel_norm, lambda v: F.channel_norm_residual(v, x, next_kind="layer")[1], lambda v: F.channel_norm_residual(x, v), lambda v: F.grad_norm([v])):
             with pytest.raises(RuntimeError):
                 transform(f)
+
+
+def test_views_that_negate_are_read_with_their_sign():
+    """The imaginary part of a conjugate holds the other sign in memory: rows (of one channel they need no copy for their strides), vectors, gates, gradients."""
+    g = torch.Generator().manual_seed(4)
+    for C in (1, 6):
+        z = torch.randn(5, C, dtype=torch.complex64, generator=g).to(DEV).conj()
+        v = torch.randn(C, dtype=torch.complex64, generator=g).to(DEV).conj()
+        x, w = z.imag, v.imag
+        assert x.is_neg() and w.is_neg()
+        plain = lambda t: t.clone().contiguous()                                                   # noqa: E731
+        for call in (lambda t, u: F.channel_norm(t, u, u, kind="rms"), lambda t, u: F.channel_norm_residual(t, t, u, kind=None, gate=u),
+                     lambda t, u: F.channel_norm_residual(t, t, u, kind="rms", gate=t, next_kind="rms", next_weight=u)[1]):
+            assert not plain(x).is_neg() and torch.equal(call(x, w), call(plain(x), plain(w)))
+            grads = []
+            for t, u, dy in ((x, w, x), (plain(x), plain(w), plain(x))):
+                leaf, vec = t.detach().requires_grad_(True), u.detach().requires_grad_(True)
+                grads.append(torch.autograd.grad(call(leaf, vec), [leaf, vec], [dy]))
+            assert all(torch.equal(a, b) for a, b in zip(*grads))
