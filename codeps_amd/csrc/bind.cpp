@@ -377,12 +377,13 @@ PyObject* py_channel_norm_residual(PyObject*, PyObject* const* a, Py_ssize_t na)
         } else {
             if (type_of(g) < 0 || g.device() != x.device() || g.dim() < 1 || g.size(-1) != c)
                 refuse(what, ": gate [..., ", c, "] in fp32, bf16 or fp16 on ", x.device(), ", got ", described(g));
+            const bool item = x.dim() > 2 && (g.dim() == 2 || g.dim() == x.dim()) && g.size(0) == x.size(0) && g.numel() == g.size(0) * c;
             if (g.dim() == 1) {
                 d.gate_mode = CODEPS_GATE_CHANNEL;
-            } else if (g.sizes() == x.sizes()) {
+            } else if (g.sizes() == x.sizes() && (g.scalar_type() == x.scalar_type() || !item)) {
                 d.gate_mode = CODEPS_GATE_ELEMENT;
                 if (g.scalar_type() != x.scalar_type()) refuse(what, ": a gate of x's shape has x's type, got ", g.scalar_type(), " for ", x.scalar_type());
-            } else if ((g.dim() == 2 || g.dim() == x.dim()) && g.size(0) == x.size(0) && g.numel() == g.size(0) * c && x.dim() > 2) {
+            } else if (item) {                                        // (items of one row each: x's shape as well, but of any type)
                 d.gate_mode = CODEPS_GATE_ITEM;
                 const int64_t rows = x.numel() / c;
                 d.rows_per_item = (int32_t)std::max<int64_t>(1, std::min<int64_t>(rows / std::max<int64_t>(1, x.size(0)), INT32_MAX));

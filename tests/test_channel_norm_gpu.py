@@ -540,3 +540,15 @@ def test_views_that_negate_are_read_with_their_sign():
                 leaf, vec = t.detach().requires_grad_(True), u.detach().requires_grad_(True)
                 grads.append(torch.autograd.grad(call(leaf, vec), [leaf, vec], [dy]))
             assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+def test_a_gate_per_item_has_a_type_of_its_own_where_an_item_is_one_row(rows):
+    """[B, 1, C] beside x [B, N, C]: with N = 1 it has x's shape too, and is a gate per item all the same."""
+    c = case(40, (3, rows), BF16, res=F32, gate="item", act="sigmoid")
+    for kept in (F32, F16, BF16):
+        t = make(c, 8)
+        t["gate"] = t["gate"].to(kept)
+        got = run(c, t)
+        assert got["dgate"].dtype == kept and got["dgate"].shape == t["gate"].shape
+        compare(c, t, got)
