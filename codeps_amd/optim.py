@@ -55,6 +55,8 @@ class AdamW:
 
     def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, small_numel=4096, ema=None, ema_alpha=0.99,
                  copies=None, max_norm=None, skip_nonfinite=False, seed=0):
+        if torch.is_tensor(params):
+            raise CodepsHipError("AdamW: a list of parameters, got one tensor (its rows would be the parameters, without its gradient)")
         params = list(params)
         if not params:
             raise CodepsHipError("AdamW: no parameters")

@@ -159,3 +159,10 @@ def test_a_trace_is_refused():
         torch.jit.trace(lambda v: v + _lib.bind().adamw_step([v], [], [v], 0, 1.0, 0.0, False, 0.9), (x,))
     with pytest.raises(CodepsHipError, match="GPU only"):             # (and nothing of it stays behind)
         F.channel_norm(x)
+
+
+def test_adamw_of_one_tensor_instead_of_a_list_is_refused():
+    """list(tensor) are views of its rows, which never have a gradient: nothing would ever move."""
+    for params in (torch.zeros(3), torch.nn.Parameter(torch.zeros(2, 3))):
+        with pytest.raises(CodepsHipError, match="a list of parameters"):
+            AdamW(params)
