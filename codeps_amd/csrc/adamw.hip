@@ -3,7 +3,7 @@
 // A step is two launches (with clipping one more, for the norm): a small one that advances every tensor's count t and turns it into the tensor's factors
 // (64 bits: 1 - b2^t of a young tensor loses its digits in 32), and the update itself.  Nothing of a step depends on host values but its scalars, so a
 // captured step replays as the next one.  The update reads and writes every byte once: 28 bytes per element with 32-bit states, 16 with 8-bit ones (fp32
-// gradients); it is bound by bandwidth: 99.6 M elements in 8 bits take 296 - 300 us (5.4 TB/s), 23.5 M in 32 bits with an average (36 bytes) 140 - 151 us
+// gradients); it is bound by bandwidth: 99.6 M elements in 8 bits take 301 us (5.3 TB/s), 23.5 M in 32 bits with an average (36 bytes) 140 - 152 us
 // (5.6 - 6.0 TB/s).
 //
 // Tensors are cut into chunks of 2048 elements, one block each; a table gives the tensor of a chunk.  The static part of a tensor (addresses, state
@@ -14,8 +14,8 @@
 //   q = floor(t / quantum + rho / 65536),  rho = 16 random bits
 // in integers: t 2^16 / quantum is below 2^21, its whole part plus rho is shifted by 16.  The fp32 value behind it is off by a unit at most, so the
 // result can differ from the exact one only where the sum lies within two units of a multiple of 65536: there (about 8 elements in 100 000) the
-// moments are formed again in 64 bits.  So are those of a whole block whose largest magnitude lies next to a border between two units (about one block in
-// 100 000).  The root is held over the whole range of fp32, but its square is not: a block goes through 64 bits as a whole, its unit
+// moments are formed again in 64 bits.  So are those of a whole block whose largest magnitude lies next to a border between two units (about two blocks
+// in 100 000).  The root is held over the whole range of fp32, but its square is not: a block goes through 64 bits as a whole, its unit
 // and the parameters' update included, where a square would overflow (roots of 2^62 or more) or lose bits that a code could see.  Those are squares below
 // 2^-120 that are not exactly zero, in blocks whose largest root is below 2^-36, or beside an eps below 2^-50: elsewhere, what a subnormal square loses (2^-74
 // of the root) is less than the 2^-16 quanta of the lowest codes (2^-70) and a rounding of the update's denominator.
@@ -226,6 +226,7 @@ __global__ __launch_bounds__(THREADS) void adamw_factors_kernel(Groups groups, c
         f.root = (float)(1.0 / sqrt(1.0 - pow(g.b2, (double)t)));
         f.eps = (float)g.eps;
         f.with64 = (gs != 0.0 && !(fabs(gs) >= 0x1p-126 && fabs(gs) < 0x1p127) ? WITH64_SCALE : 0) | (f.eps >= f.root * 0x1p-50f ? 0 : WITH64_ROOT);
+        // keys: the 64-bit finaliser of Steele, Lea and Flood, "Fast splittable pseudorandom number generators" (2014), over seed, step and tensor
         unsigned long long z = seed + (unsigned long long)t * 0x9E3779B97F4A7C15ull + (unsigned long long)(base + i) * 0xD1B54A32D192ED03ull;
         z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
         z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
@@ -269,6 +270,7 @@ template <int MANT> __device__ __forceinline__ unsigned unit64(double a) {
     const unsigned e = (unsigned)(((unsigned long long)__double_as_longlong(a) + ((1ull << (52 - MANT)) - 1)) >> 52) - (1023 - 127);
     return a < 0x1p-126 ? 0u : min(e, 255u);
 }
+// 32 random bits of an element: a multiply-xorshift mix of two rounds (shifts and multipliers of Wellons's search for low-bias 32-bit hashes), keyed per tensor and step
 __device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsigned k1) {
     unsigned x = (unsigned)i + (unsigned)(i >> 32) * 0x9E3779B1u + k0;
     x = (x ^ (x >> 16)) * 0x7FEB352Du;
@@ -303,7 +305,8 @@ __device__ __forceinline__ void moments64(const Factors& f, double m0, double r0
     v = c + d;
 }
 
-// one chunk of a tensor; WIDE: 32-bit states.  The gradients are loaded last: their type is known at run time, and where the branches meet the compiler waits.
+// One chunk of a tensor; WIDE: 32-bit states.  The update divides by a reciprocal that is off by a step (2^-23 of the update, one of the handful of roundings
+// that it takes in fp32), an 8-bit root is a square root off by a step, which the two units of `encode` allow for.  The gradients are loaded last: their type is known at run time, and where the branches meet the compiler waits.
 template <bool WIDE, bool TAIL>
 __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, const void* gp, int gt, float* const ema, long long start, const States& st, float al, float oal) {
     constexpr int K = CHUNK / (THREADS * 4);

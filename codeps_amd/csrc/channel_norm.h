@@ -188,8 +188,8 @@ template <bool BLOCK> __device__ __forceinline__ Place place_of(int lpr_log2) {
 }
 
 // The slice of a block.  Blocks go to the 8 XCDs in turn.  Where a row is not a whole number of 128-byte lines, neighbouring slices, whose rows share lines, are
-// given to blocks of one XCD, and its L2 merges their parts of a line: 32768 x 1000 bf16, forward and backward 87 -> 82 us; whole lines are better off in
-// turn (262144 x 256 bf16 131 against 137 us).
+// given to blocks of one XCD, and its L2 merges their parts of a line: norm alone, bf16, forward and backward, 32768 x 1000 86 -> 82 us, 32768 x 1001 109 -> 106;
+// whole lines are better off in turn (262144 x 256 132 against 137 us).
 __device__ __forceinline__ int slice_of(unsigned block, int S, bool shared_lines) {
     const int s = (int)(block % (unsigned)S);
     return shared_lines && S % 8 == 0 ? (s & 7) * (S >> 3) + (s >> 3) : s;
@@ -290,7 +290,7 @@ inline Shape shape_of(const codeps_channel_norm_desc* d) {
     return s;
 }
 // Blocks work on rows of one item (the rows that share an ITEM gate; all rows otherwise): block (item, slice) takes every slices-th group of rows, so that the
-// chip walks through memory in step (contiguous ranges per block: the stride-4 norm's backward pass 98 instead of 77 us).  Blocks loop over items.
+// chip walks through memory in step (contiguous ranges per block: norm alone, 262144 x 256 bf16, backward kernel 98 instead of 77 us).  Blocks loop over items.
 inline bool shared_lines(const codeps_channel_norm_desc* d) { return d->channels * (d->x_type == CODEPS_F32 ? 4 : 2) % 128 != 0; }
 struct Plan { Shape s; int items, rpi, slices, blocks; };
 inline Plan plan_of(const codeps_channel_norm_desc* d, int want, int resident) {

@@ -40,15 +40,19 @@ template <int V, int NCH, typename TX, typename TR, bool ROWS> struct Row {
     float4 st;                                       // mean and 1 / deviation of both norms
 };
 
-// Rows of more than 4096 channels take blocks of more than 512 threads, which have 128 registers each.  SUMS_WIDE: the column sums fit there (norm alone, 16-bit
-// block ends without a gate): 4096 x 8192 bf16, norm alone, 108 us, forward and backward, with a pass of their own 139; 4096 x 5000 with residual and next norm
-// 175 / 204 us.  SUMS_APART: they would spill (16-bit rows around an fp32 residual 190 -> 212 us, a gate per element 190 -> 207, per channel 180 -> 263):
-// channel_norm_columns_kernel forms them from the row's two sums of n'^T.
+// Times below are forward and backward together, bf16 in and out, layer norms with weight and bias, "next": with the next block's norm.
+//
+// Rows of more than 4096 channels take blocks of more than 512 threads, which have 128 registers each.  SUMS_WIDE: the column sums fit there (norm alone; 16-bit
+// block ends without a gate: 4096 x 5000, next, 175 us, apart 204).  SUMS_APART: channel_norm_columns_kernel forms them from the row's two sums of n'^T.  In place
+// they spill 8 - 276 bytes (4096 x 5000, next: around an fp32 residual 228 -> 250 us, a gate per element 250 -> 273, per channel 272 -> 392); fp32 rows
+// without a gate would bear it (4096 x 8192, next, 442 -> 416), but no kernel here uses scratch.
 //
 // Loads of a row are issued together, before anything is widened.  AHEAD: those of the next row as well, before the current one's arithmetic: for gates held over
-// 16-bit rows, where the sums' registers allow two waves per SIMD either way (forward and backward: 20485 x 768 bf16 around an fp32 residual 117 -> 115 us,
-// 8192 x 4096 bf16 233 -> 214, 32768 x 2048 354 -> 336), and for a norm alone in wide rows, where one block fills a CU (4096 x 8192 bf16 120 -> 108 us).
-// Elsewhere it costs a wave (65536 x 1024 bf16 without gate 297 -> 340 us) or gains nothing (fp32 rows).
+// 16-bit rows, where the sums' registers allow two waves per SIMD either way, and for a norm alone in wide rows, where one block fills a CU (4096 x 8192
+// 117 -> 102 us).  Held gates: 8192 x 4096, channel gate, next, 233 -> 214 us; 32768 x 2048, channel gate, next, 352 -> 333, without next 218 -> 190;
+// 20485 x 768 around an fp32 residual, item gate, next, 117 -> 114; but 32768 x 2048 around fp32, channel gate, next, 392 -> 413.  (Three waves per SIMD without
+// it spill; 32768 x 2048, channel gate, next, took 316 us that way.)  Elsewhere it costs a wave or scratch (gate per element, next, 32768 x 1024 203 -> 239;
+// 4096 x 5000, next, 175 -> 235) or gains nothing (65536 x 1024, next, 300 -> 303; fp32 rows 273 -> 274).
 template <typename TX, bool BLOCK, bool FULL, int GATE, int SUMS> struct Form {
     static constexpr bool held = BLOCK && SUMS == SUMS_HERE && GATE == GATE_HELD;
     static constexpr bool ahead = (held && sizeof(TX) == 2) || (SUMS == SUMS_WIDE && !FULL);
@@ -393,9 +397,10 @@ __global__ __launch_bounds__(16 * FINISH_STREAMS) void channel_norm_finish_kerne
 }
 
 // Blocks: as many as are resident at once, by the registers of the kernel that runs -- more leave a tail of late blocks, fewer leave lanes idle.  Forward and
-// backward together at 8 / 12 / 16 waves per CU, us: norm alone, 65536 x 768 bf16 146 / 125 / 117, 16384 x 2048 fp32 131 / 133 / 140; block end in one 16-bit
-// type, 65536 x 1024 with an added norm 290 / 275 / 283; 16-bit blocks around an fp32 residual, 32768 x 2048 389 / 396 / 424, 20485 x 768 with an item gate
-// 115 / 128 / 133; all fp32, 20485 x 768 with an item gate 151 / 171 / 184, 32768 x 1024 274 / 279 / 292.
+// backward together at 8 / 12 / 16 waves per CU, us: norm alone, 65536 x 768 bf16 147 / 127 / 119, 16384 x 2048 fp32 130 / 132 / 138; block end in one 16-bit
+// type, next norm, no gate, 65536 x 1024 327 / 300 / 308, gate per element, 32768 x 1024 217 / 202 / 224, channel gate, 65536 x 1024 330 / 380 / 396; 16-bit blocks
+// around an fp32 residual, next norm, 32768 x 2048, channel gate 416 / 422 / 422, 20485 x 768, item gate 114 / 127 / 133; all fp32, next norm, 20485 x 768, item gate
+// 152 / 174 / 185, 32768 x 1024, channel gate 272 / 294 / 319.
 // A block takes at least 8 rows per row group where there are that many: its column sums' slab is a cost of its own.
 Plan bwd_plan(const codeps_channel_norm_desc* d) {
     const Shape s = shape_of(d);

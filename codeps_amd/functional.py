@@ -2374,7 +2374,8 @@ def channel_norm_residual(x, residual=None, weight=None, bias=None, *, kind="lay
     Returns y, or (y, h) with next_kind.  x [..., C] is the block's output; kind None leaves it as it is (times weight, plus bias, if given).
     residual: x's shape, x's type or fp32 (a residual stream in 32 bits around 16-bit blocks); y has its type, h has x's.  None: zeros.
     gate: [C] (layer scale), one row per item of the first dimension ([B, C], or x's number of dimensions with ones in between), or x's shape (and type);
-    gate_act: None, "sigmoid" (1 and 0 at +inf and -inf) or "silu" (g sigmoid(g): inf at +inf, NaN at -inf).  scale: a float.  h is the norm of y before y is rounded to its type."""
+    gate_act: None, "sigmoid" (1 and 0 at +inf and -inf) or "silu" (g sigmoid(g): inf at +inf, NaN at -inf).  scale: a float.  h is the norm of y before y is
+    rounded to its type."""
     if kind not in _NORM_KINDS or next_kind not in _NORM_KINDS:
         raise CodepsHipError(f"channel_norm_residual: kind and next_kind are \"layer\", \"rms\" or None, got {kind!r} and {next_kind!r}")
     if gate_act not in _GATE_ACTS:

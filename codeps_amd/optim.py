@@ -43,6 +43,8 @@ def _same_layout(a, b):
 class AdamW:
     """m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
 
+    Not a torch.optim.Optimizer: torch's learning-rate schedulers do not take it.  Set param_groups[i]["lr"] between steps, or give a device scalar.
+
     params: fp32 tensors on one device, or dicts {"params": [...]} with their own lr, betas, eps, weight_decay, state_bits (at most 16).
         Parameters in 16 bits would lose every update below half a step: keep them in fp32 and ask for `copies`.
     lr: a float, or an fp32 device scalar that the step reads when it runs (schedules inside a captured graph).
