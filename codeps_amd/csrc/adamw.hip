@@ -388,25 +388,34 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 deep = __builtin_amdgcn_ballot_w64(deep) != 0;
             }
             unsigned ncm = 0, ncr = 0;
-            if (__builtin_expect(unsure || deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE), false)) {                // the same for the whole wave
-                double m[4], r[4];
-                unsigned tm = 0, tr = 0;
+            if (__builtin_expect(unsure || deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE), false)) {          // the same for the whole wave
+                // (a block of zeros, states and gradients: what a row without gradients keeps is 10 % of the whole step in 64 bits)
+                bool some = ((mc[k] & 0x7f7f7f7fu) | rc[k]) != 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    double v;
-                    moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m[e], v);
-                    r[e] = sqrt(v);
-                    p[k][e] = (float)((double)p[k][e] * f.keep - (double)f.rate * m[e] / (r[e] * f.root + f.eps));
-                    tm = max(tm, unit64<MANT_M>(fabs(m[e])));
-                    tr = max(tr, unit64<MANT_R>(r[e]));
-                }
-                nm = (int)wave_umax(tm);
-                nr = (int)wave_umax(tr);
+                for (int e = 0; e < 4; ++e) some = some || g[k][e] != 0.f;
+                if (nm == 0 && nr == 0 && f.eps > 0.f && __builtin_amdgcn_ballot_w64(some) == 0) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned rnd = random_bits(i + e, f.k0, f.k1);
-                    ncm |= (encode64<MANT_M>(fabs(m[e]), nm, rnd & 0xffffu) | (m[e] < 0.0 ? 128u : 0u)) << (8 * e);
-                    ncr |= encode64<MANT_R>(r[e], nr, rnd >> 16) << (8 * e);
+                    for (int e = 0; e < 4; ++e) p[k][e] *= f.keep;
+                } else {
+                    double m[4], r[4];
+                    unsigned tm = 0, tr = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        double v;
+                        moments64(f, (double)m0[e], (double)r0[e], (double)g[k][e], m[e], v);
+                        r[e] = sqrt(v);
+                        p[k][e] = (float)((double)p[k][e] * f.keep - (double)f.rate * m[e] / (r[e] * f.root + f.eps));
+                        tm = max(tm, unit64<MANT_M>(fabs(m[e])));
+                        tr = max(tr, unit64<MANT_R>(r[e]));
+                    }
+                    nm = (int)wave_umax(tm);
+                    nr = (int)wave_umax(tr);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned rnd = random_bits(i + e, f.k0, f.k1);
+                        ncm |= (encode64<MANT_M>(fabs(m[e]), nm, rnd & 0xffffu) | (m[e] < 0.0 ? 128u : 0u)) << (8 * e);
+                        ncr |= encode64<MANT_R>(r[e], nr, rnd >> 16) << (8 * e);
+                    }
                 }
             } else {
 #pragma unroll

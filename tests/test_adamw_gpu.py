@@ -736,3 +736,26 @@ def test_gradients_that_negate_on_reading():
         for bad in (lambda: AdamW([g[:1]]), lambda: AdamW([p[:1]], ema=[g[:1]])):
             with pytest.raises(CodepsHipError):
                 bad()
+
+
+def test_rows_without_gradients_in_eight_bits():
+    """Blocks whose states and gradients are zeros, between others: they decay with the weight decay and keep zeros; they take part again as soon as a gradient comes,
+    and stay in it when it goes.  Without an eps the formula is 0 / 0 there."""
+    params = tensors([4096, 300], 6)
+    opt = AdamW(params, lr=1e-2, weight_decay=0.1, state_bits=8, small_numel=1, seed=8)
+    plain = Plain(params, [0.1] * 2, [8] * 2, 1e-2, (0.9, 0.999), 1e-8, seed=8)
+    for k in range(4):
+        grads = gradients(params, 80 + k)
+        rows = grads[0].view(16, 256)
+        rows[0], rows[3], rows[9:12], rows[15, :255] = 0.0, -0.0, 0.0, 0.0
+        if k in (0, 2):
+            rows[5], grads[1][:256] = 0.0, 0.0
+        opt.step(grads)
+        plain.step(grads)
+        check(opt, plain)
+        assert opt.exp_avg_exponents[0] == 0 and not opt.exp_avg_codes[:256].any() and not opt.root_codes[:256].any()
+    q = torch.ones(512, device=DEV)
+    g = torch.zeros(512, device=DEV)
+    g[256:] = 1.0
+    AdamW([q], lr=1e-2, eps=0.0, state_bits=8, small_numel=1).step([g])
+    assert torch.isnan(q[:256]).all() and torch.isfinite(q[256:]).all()
