@@ -3,7 +3,7 @@
 // A step is two launches (with clipping one more, for the norm): a small one that advances every tensor's count t and turns it into the tensor's factors
 // (64 bits: 1 - b2^t of a young tensor loses its digits in 32), and the update itself.  Nothing of a step depends on host values but its scalars, so a
 // captured step replays as the next one.  The update reads and writes every byte once: 28 bytes per element with 32-bit states, 16 with 8-bit ones (fp32
-// gradients); it is bound by bandwidth: 99.6 M elements in 8 bits take 301 us (5.3 TB/s), 23.5 M in 32 bits with an average (36 bytes) 140 - 152 us
+// gradients); it is bound by bandwidth: 99.6 M elements in 8 bits take 301 - 309 us (5.2 - 5.3 TB/s), 23.5 M in 32 bits with an average (36 bytes) 140 - 153 us
 // (5.6 - 6.0 TB/s).
 //
 // Tensors are cut into chunks of 2048 elements, one block each; a table gives the tensor of a chunk.  The static part of a tensor (addresses, state

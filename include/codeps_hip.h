@@ -539,7 +539,7 @@ int codeps_channel_norm_bwd(const codeps_channel_norm_desc* d, const void* x, co
  * zeros), `state_offset` a multiple of 256: m as sign / 4 exponent / 3 mantissa bits, sqrt(v) as 4 exponent / 4 mantissa bits, each block with one
  * biased exponent byte: value = (-1)^s f 2^(byte - 127), f = mantissa 2^(-14 - mant_bits) for exponent field 0, else (1 + mantissa 2^-mant_bits)
  * 2^(field - 15); the block's exponent is the smallest under which its largest magnitude fits; byte 0: zeros (nothing of 2^-126 or more), byte 255:
- * not finite (decodes as NaN).  Codes are rounded to one of the two neighbours with the odds of the place between them, by 16 random bits of
+ * not finite, or too large for byte 254 (decodes as NaN).  Codes are rounded to one of the two neighbours with the odds of the place between them, by 16 random bits of
  * (seed, tensor's index, t, element): rounding to nearest would lose an average's steps, which are far below half a code.  The parameter's update uses
  * m and v before they are rounded.
  * Usage: host buffer of n * codeps_adamw_item_bytes(), one codeps_adamw_item_fill per tensor in order (returns the tensor's number of chunks, negative
