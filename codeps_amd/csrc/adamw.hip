@@ -220,7 +220,7 @@ __global__ __launch_bounds__(THREADS) void adamw_factors_kernel(Groups groups, c
         f.live = live; f.skipped = skip;
         f.b1 = g.b1; f.ob1 = 1.0 - g.b1; f.b2 = g.b2; f.ob2 = 1.0 - g.b2; f.gs = gs;
         f.fb1 = (float)f.b1; f.fob1 = (float)f.ob1; f.fb2 = (float)f.b2; f.fob2 = (float)f.ob2; f.fgs = (float)gs;
-                const double lr = g.lr_dev ? (double)*g.lr_dev : g.lr;
+        const double lr = g.lr_dev ? (double)*g.lr_dev : g.lr;
         f.keep = (float)(1.0 - lr * g.wd);
         f.rate = (float)(lr / (1.0 - pow(g.b1, (double)t)));
         f.root = (float)(1.0 / sqrt(1.0 - pow(g.b2, (double)t)));
@@ -270,7 +270,8 @@ template <int MANT> __device__ __forceinline__ unsigned unit64(double a) {
     const unsigned e = (unsigned)(((unsigned long long)__double_as_longlong(a) + ((1ull << (52 - MANT)) - 1)) >> 52) - (1023 - 127);
     return a < 0x1p-126 ? 0u : min(e, 255u);
 }
-// 32 random bits of an element: a multiply-xorshift mix of two rounds (shifts and multipliers of Wellons's search for low-bias 32-bit hashes), keyed per tensor and step
+// 32 random bits of an element: a multiply-xorshift mix of two rounds (shifts and multipliers of Wellons's search for low-bias 32-bit hashes), keyed per tensor
+// and step
 __device__ __forceinline__ unsigned random_bits(long long i, unsigned k0, unsigned k1) {
     unsigned x = (unsigned)i + (unsigned)(i >> 32) * 0x9E3779B1u + k0;
     x = (x ^ (x >> 16)) * 0x7FEB352Du;
@@ -306,7 +307,8 @@ __device__ __forceinline__ void moments64(const Factors& f, double m0, double r0
 }
 
 // One chunk of a tensor; WIDE: 32-bit states.  The update divides by a reciprocal that is off by a step (2^-23 of the update, one of the handful of roundings
-// that it takes in fp32), an 8-bit root is a square root off by a step, which the two units of `encode` allow for.  The gradients are loaded last: their type is known at run time, and where the branches meet the compiler waits.
+// that it takes in fp32), an 8-bit root is a square root off by a step, which the two units of `encode` allow for.  The gradients are loaded last: their type is
+// known at run time, and where the branches meet the compiler waits.
 template <bool WIDE, bool TAIL>
 __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, const void* gp, int gt, float* const ema, long long start, const States& st, float al, float oal) {
     constexpr int K = CHUNK / (THREADS * 4);
@@ -388,7 +390,8 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Factors& f, c
                 deep = __builtin_amdgcn_ballot_w64(deep) != 0;
             }
             unsigned ncm = 0, ncr = 0;
-            if (__builtin_expect(unsure || deep || nm < 14 || nr < 14 || nm == 255 || nr > 189 || (f.with64 & WITH64_SCALE), false)) {          // the same for the whole wave
+            const bool ends = nm < 14 || nr < 14 || nm == 255 || nr > 189;
+            if (__builtin_expect(unsure || deep || ends || (f.with64 & WITH64_SCALE), false)) {      // the same for the whole wave
                 // (a block of zeros, states and gradients: what a row without gradients keeps is 10 % of the whole step in 64 bits)
                 bool some = ((mc[k] & 0x7f7f7f7fu) | rc[k]) != 0;
 #pragma unroll

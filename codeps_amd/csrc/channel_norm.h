@@ -248,8 +248,8 @@ template <int V, bool TAIL, bool ZEROS> __device__ __forceinline__ float piece_s
     return TAIL || left > 0 ? s : 0.f;
 }
 
-// 1 / (1 + exp(-g)) on the hardware's 2^x and reciprocal (1 step each); the rounding of g log2(e) is carried along, or it would cost |g| steps.  It is below 1
-// wherever it matters; the minimum is for g = +inf and finite gates whose product overflows, where it is infinite or NaN beside e = 0 (the gate is 1 there).
+// 1 / (1 + exp(-g)) on the hardware's 2^x and reciprocal (1 step each); the rounding of g log2(e) is carried along, or it would cost |g| steps.  That
+// rounding, lo, is far below 1 while e counts; for g = +inf and finite gates whose product overflows it is infinite or NaN beside e = 0, hence the minimum.
 __device__ __forceinline__ float sigmoid(float g) {
     const float hi = g * -1.44269504f, lo = __builtin_fmaf(g, -1.44269504f, -hi) + g * -1.92596299e-8f;
     const float e = __builtin_amdgcn_exp2f(hi), t = __builtin_fmaf(e, fminf(lo, 1.f) * 0.69314718f, e);
